@@ -199,6 +199,33 @@ int omc_splice(const int64_t* ids, const int32_t* seq_offsets, int n_seq, int S_
  * (lowest index on ties), logits fp32 [B, V] with row stride ldl. workspace: 128*B floats. */
 int omc_argmax(const float* logits, long long ldl, int B, int V, int64_t* next, float* workspace, void* stream);
 
+/* ---- going on with cached sequences by a chunk of new tokens (omchat_b200/csrc/rotary.cu, chunk_attention.cu) ------------------
+ * Rotary positions (transformers modeling_qwen2.py:102-146 and its scaled kinds). x [T, heads * head_dim] -> y (may be x), bf16 or (fp32 != 0)
+ * fp32 rows, leading dims in elements. Of every head the first rot_dims (even, <= head_dim <= 256) dimensions are rotated by the row's
+ * position, i with i + rot_dims / 2 (halves != 0) or 2i with 2i + 1; the others are copied. turns: float64 [rot_dims / 2] in device memory, the
+ * frequencies in turns per position (inverse frequency / 2 pi); the angle is formed in 64 bits. Cosine and sine are multiplied by mscale.
+ * back != 0: by the negative angle (the inverse for mscale 1, the gradient for any). Any alignment; 16-byte rows and rot_dims a multiple of 16 are the fast way. */
+int omc_rotary_rows(const void* x, int fp32, long long ldx, const int32_t* pos, int T, int heads, int head_dim, const double* turns, int rot_dims,
+                    int halves, int back, float mscale, void* y, long long ldy, void* stream);
+/* The rows of a step before its attention: qkv bf16 [T, (Hq + 2 Hkv) * head_dim] holds q | k | v; q is rotated into q_out [T, Hq * head_dim] (may be
+ * qkv's own columns), k is rotated and v copied into the cache, kv_pool bf16 [n_pages, 2, Hkv, page_size, head_dim] (page = block_table[seq_ids[t]][pos[t] /
+ * page_size], int32 [n_seq][max_pages]). seq_ids NULL: all rows belong to sequence 0. A row whose sequence, position or page is outside the table or the
+ * pool is not appended (a row of padding has sequence -1). No two rows of a call may have the same place. page_size: any. */
+int omc_rotary_kv_append(const void* qkv, long long ldqkv, const int32_t* pos, const int32_t* seq_ids, int T, int Hq, int Hkv, int head_dim,
+                         const double* turns, int rot_dims, int halves, float mscale, void* q_out, long long ldq, void* kv_pool, int n_pages,
+                         const int32_t* block_table, int n_seq, int max_pages, int page_size, void* stream);
+/* Causal attention of n new tokens per sequence (1 and more, 0 for a sequence without any) over the cache, which holds them already: the rows
+ * cu_new[s] .. cu_new[s + 1] - 1 (int32 [n_seq + 1]) of q and out (bf16, [T, Hq * head_dim], head_dim 64 or 128) are the last n of the ctx_lens[s] positions of
+ * sequence s, and row i of them sees the keys 0 .. ctx_lens[s] - n + i. A row that sees none is zero; rows behind cu_new[n_seq] are left as they are.
+ * max_new and max_ctx: what no sequence has more of (rows beyond max_new are not computed, positions beyond max_ctx or the table not read); the device reads
+ * the lengths itself, so a captured call goes by the lengths of its replay. Pages outside the pool read as zeros. Keys and values behind ctx_lens[s] may
+ * hold anything; a value that is not finite reaches the rows of its sequence that are computed beside those that see it (as many as share a tile).
+ * workspace: omc_paged_chunk_attn_workspace_bytes(...) bytes (0: NULL is fine), 16-byte aligned, nothing in it outlives the call. */
+long long omc_paged_chunk_attn_workspace_bytes(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim);
+int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv_pool, int n_pages, const int32_t* block_table, int max_pages, int page_size,
+                         const int32_t* cu_new, const int32_t* ctx_lens, int n_seq, int T, int max_new, int max_ctx, int Hq, int Hkv, int head_dim,
+                         float scale, void* out, long long ldo, void* workspace, long long workspace_bytes, void* stream);
+
 /* ---- weight-streaming GEMM of the batched decode step (omchat_b200/csrc/gemm_stream.cu) --------------------------------
  * Replaces, for M <= 64 rows, the nn.Linear calls of Qwen2Attention / Qwen2MLP / lm_head (transformers modeling_qwen2.py:
  * 46-48, 219-221, 245, 470-472) together with the Qwen2RMSNorm in front of them (:258-263): Y[M,N] = epi(rstd[m] * (X W'^T)).

@@ -1,0 +1,139 @@
+// Rotary positions of rows of heads, and the append of keys and values to the paged cache with the rotation on the way.
+//
+// Of every head the first `rot` dimensions are rotated pairwise, dimension i with i + rot / 2 (halves) or 2i with 2i + 1:
+//   (u, v) -> (u c - v s, v c + u s),  c = m cos(2 pi a), s = m sin(2 pi a),  a = position * turns[i]
+// turns[i] is the pair's frequency in turns per position. The angle is formed and reduced to a part of one turn in 64 bits: at position 10^5
+// a 32-bit product is off by up to 0.01 radians, a bf16 step of the result. Frequencies stretched for long contexts are other numbers in `turns`,
+// and a factor m where the method has one.
+#include <stdint.h>
+
+#include "omc_internal.h"
+#include "ptx.cuh"
+
+namespace omc {
+
+typedef __nv_bfloat16 bf16;
+
+struct RotaryArgs {
+  const void* x;
+  long long ldx;
+  void* y;                 // rotated heads (with a cache: the query heads)
+  long long ldy;
+  const int32_t* pos;
+  const int32_t* seq;      // row of the table; NULL: row 0
+  const double* turns;
+  int T, turned, heads, head, rot, halves;   // of `heads` heads of a row the first `turned` are rotated
+  float m, sign;
+  bf16* pool;              // [n_pages][2][hkv][page_size][head] or NULL: heads from hq on go there
+  const int32_t* table;
+  int hq, hkv, n_seq, max_pages, page_size, n_pages;
+};
+
+__device__ __forceinline__ float rotary_load(const float* p) { return *p; }
+__device__ __forceinline__ float rotary_load(const bf16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void rotary_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rotary_store(bf16* p, float v) { *p = __float2bfloat16(v); }
+
+// (cos, sin) of pair i at position p.
+__device__ __forceinline__ float2 rotary_factor(const RotaryArgs& a, int p, int i) {
+  double turn = (double)p * a.turns[i];
+  turn -= rint(turn);
+  float s, c;
+  sincospif((float)(2.0 * turn), &s, &c);
+  return make_float2(c * a.m, s * a.m * a.sign);
+}
+
+// First element of the pool's row for (keys 0 or values 1, head 0) of row t, or -1 where the row has no place in the cache.
+__device__ __forceinline__ long long rotary_place(const RotaryArgs& a, int t) {
+  const int p = a.pos[t], s = a.seq != nullptr ? a.seq[t] : 0;
+  if (s < 0 || s >= a.n_seq || p < 0 || p / a.page_size >= a.max_pages) return -1;
+  const int page = a.table[(long long)s * a.max_pages + p / a.page_size];
+  if (page < 0 || page >= a.n_pages) return -1;
+  return ((long long)page * 2 * a.hkv * a.page_size + p % a.page_size) * a.head;
+}
+
+template <typename TT>
+__global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a) {
+  const int t = blockIdx.x, half = a.rot / 2;
+  __shared__ float2 cs[128];
+  for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i] = rotary_factor(a, a.pos[t], i);
+  __syncthreads();
+  const TT* row = static_cast<const TT*>(a.x) + t * a.ldx;
+  TT* out = static_cast<TT*>(a.y) + t * a.ldy;
+  const long long place = a.pool != nullptr ? rotary_place(a, t) : 0;
+  for (int e = threadIdx.x; e < a.heads * a.head; e += blockDim.x) {
+    const int h = e / a.head, d = e - h * a.head;
+    const TT* src = row + h * a.head;
+    TT* dst;
+    if (a.pool == nullptr || h < a.hq) {
+      dst = out + h * a.head;
+    } else {
+      if (place < 0) continue;
+      dst = reinterpret_cast<TT*>(a.pool) + place + (long long)(h - a.hq) * a.page_size * a.head;   // key heads, then value heads: [2][hkv] in a page
+    }
+    if (h >= a.turned || d >= a.rot) {
+      rotary_store(dst + d, rotary_load(src + d));
+      continue;
+    }
+    if (d >= half) continue;
+    const int iu = a.halves ? d : 2 * d, iv = a.halves ? d + half : 2 * d + 1;
+    const float u = rotary_load(src + iu), v = rotary_load(src + iv);
+    rotary_store(dst + iu, u * cs[d].x - v * cs[d].y);
+    rotary_store(dst + iv, v * cs[d].x + u * cs[d].y);
+  }
+}
+
+static int rotary_launch(const RotaryArgs& a, bool fp32, cudaStream_t st) {
+  if (fp32) rotary_rows_kernel<float><<<a.T, 256, 0, st>>>(a);
+  else rotary_rows_kernel<bf16><<<a.T, 256, 0, st>>>(a);
+  return check_launch("omc_rotary");
+}
+
+static int rotary_check(int T, int head, int rot, const double* turns) {
+  if (T < 0) return set_error(OMC_ERR_SHAPE, "omc_rotary: negative number of rows");
+  if (head <= 0 || head > 256 || rot < 0 || rot > head || rot % 2 != 0)
+    return set_error(OMC_ERR_SHAPE, "omc_rotary: heads of 1 to 256, of which an even number of dimensions is rotated");
+  if (rot > 0 && turns == nullptr) return set_error(OMC_ERR_ARG, "omc_rotary: no frequencies");
+  return OMC_OK;
+}
+
+}  // namespace omc
+
+using namespace omc;
+
+extern "C" int omc_rotary_rows(const void* x, int fp32, long long ldx, const int32_t* pos, int T, int heads, int head_dim, const double* turns, int rot_dims,
+                               int halves, int back, float mscale, void* y, long long ldy, void* stream) {
+  const int rc = rotary_check(T, head_dim, rot_dims, turns);
+  if (rc != OMC_OK) return rc;
+  if (heads <= 0) return set_error(OMC_ERR_SHAPE, "omc_rotary_rows: no heads");
+  if (T == 0) return OMC_OK;
+  if (x == nullptr || y == nullptr || pos == nullptr) return set_error(OMC_ERR_ARG, "omc_rotary_rows: null pointer");
+  if (T > 1 && (ldx < (long long)heads * head_dim || ldy < (long long)heads * head_dim))
+    return set_error(OMC_ERR_SHAPE, "omc_rotary_rows: rows overlap");
+  RotaryArgs a{};
+  a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.pos = pos; a.turns = turns;
+  a.T = T; a.turned = a.heads = a.hq = heads; a.head = head_dim; a.rot = rot_dims; a.halves = halves != 0;
+  a.m = mscale; a.sign = back != 0 ? -1.f : 1.f;
+  return rotary_launch(a, fp32 != 0, (cudaStream_t)stream);
+}
+
+extern "C" int omc_rotary_kv_append(const void* qkv, long long ldqkv, const int32_t* pos, const int32_t* seq_ids, int T, int Hq, int Hkv, int head_dim,
+                                    const double* turns, int rot_dims, int halves, float mscale, void* q_out, long long ldq, void* kv_pool, int n_pages,
+                                    const int32_t* block_table, int n_seq, int max_pages, int page_size, void* stream) {
+  const int rc = rotary_check(T, head_dim, rot_dims, turns);
+  if (rc != OMC_OK) return rc;
+  if (Hq <= 0 || Hkv <= 0) return set_error(OMC_ERR_SHAPE, "omc_rotary_kv_append: no heads");
+  if (n_pages <= 0 || n_seq <= 0 || max_pages <= 0 || page_size <= 0) return set_error(OMC_ERR_ARG, "omc_rotary_kv_append: bad paging parameters");
+  if (T == 0) return OMC_OK;
+  if (qkv == nullptr || q_out == nullptr || pos == nullptr || kv_pool == nullptr || block_table == nullptr)
+    return set_error(OMC_ERR_ARG, "omc_rotary_kv_append: null pointer");
+  if (T > 1 && (ldqkv < (long long)(Hq + 2 * Hkv) * head_dim || ldq < (long long)Hq * head_dim))
+    return set_error(OMC_ERR_SHAPE, "omc_rotary_kv_append: rows overlap");
+  RotaryArgs a{};
+  a.x = qkv; a.ldx = ldqkv; a.y = q_out; a.ldy = ldq; a.pos = pos; a.seq = seq_ids; a.turns = turns;
+  a.T = T; a.turned = Hq + Hkv; a.heads = Hq + 2 * Hkv; a.head = head_dim; a.rot = rot_dims; a.halves = halves != 0;
+  a.m = mscale; a.sign = 1.f;
+  a.pool = static_cast<bf16*>(kv_pool); a.table = block_table;
+  a.hq = Hq; a.hkv = Hkv; a.n_seq = n_seq; a.max_pages = max_pages; a.page_size = page_size; a.n_pages = n_pages;
+  return rotary_launch(a, false, (cudaStream_t)stream);
+}
