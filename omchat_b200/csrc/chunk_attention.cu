@@ -1,16 +1,38 @@
-// Attention of a chunk of new tokens over the paged cache, which holds the new tokens' keys and values already.
+// Attention of a chunk of new tokens over the paged cache, which holds the new tokens' keys and values already, on tcgen05 / TMEM.
 //
 // Sequence s has the rows cu[s] .. cu[s + 1] - 1 of q, at the positions ctx[s] - n .. ctx[s] - 1 of its cache (n rows):
 //   o[t, h] = sum_{j <= p(t)} softmax_j(scale q[t, h] . k[j, g]) v[j, g],  g = h / (Hq / Hkv)
+//
+// Rows are the (token, query head) pairs of one key/value head, token by token, so that a tile of keys is read once for all heads of a group and a single
+// token of 28 heads on 4 is a tile of 7 rows. A block is 256 rows of a sequence and a key/value head, a tile 128 keys.
+//   two streams of 128 rows take turns on the tensor pipe: S = Q K^T into TMEM, softmax in registers (a thread per row, running maximum and sum), P back to
+//   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. While one stream is in its softmax the pipe works for the other.
+//   A block of at most 128 rows (all of a step of single tokens) gives its one tile of queries to both streams, which take every other tile of keys and are
+//   merged at the end: the rows of a stream lie on the same lanes of TMEM.
+// One CTA per SM walks over its share of the work: the products of all blocks (128 rows x 128 keys) in one line, cut into equal parts whatever the
+// lengths are, at a tile of keys. Each CTA finds its part from cu and ctx by itself. A block that is cut leaves its parts (unnormalised O, maximum, sum; two at
+// most per CTA) in the workspace, and a second kernel, launched early, joins them.
+//   warps 0..3    keys and values by cp.async (rows through the page table, any page size), a ring of tiles
+//   warps 4..11   softmax and epilogue of the two streams
+//   warp 12       MMA issuer (one thread)
+//   warps 13..15  queries
+// Keys behind a block's last are zero-filled, so what a page holds behind a context meets no product.
 #include <math.h>
 #include <stdint.h>
 
 #include "omc_internal.h"
-#include "ptx.cuh"
+#include "sm100_step.cuh"
 
 namespace omc {
 
 typedef __nv_bfloat16 bf16;
+
+constexpr int kCaRows = 128, kCaKeys = 128, kCaBlock = 256, kCaThreads = 512, kCaBox = 128 * 128;   // kCaBox: bytes of 64 columns x 128 rows
+constexpr int kCaMinUnits = 4;           // products (128 rows x 128 keys) a CTA has at least
+constexpr int kCaJoinRows = 8;
+constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
+
+static __device__ unsigned int g_chunk_failures;   // waits that ran out
 
 struct ChunkArgs {
   const bf16* q;
@@ -23,58 +45,715 @@ struct ChunkArgs {
   long long ldo;
   int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, Hq, Hkv;
   float scale_log2;
+  int4* head;              // workspace: [CTAs] (flags, first row of q, first row of the block, rows | key/value head << 16)
+  float2* ml;              // [2 CTAs][part_rows] maximum (base 2, scaled) and sum
+  float* part;             // [2 CTAs][part_rows][D]
+  int part_rows;
+  unsigned int* failed;
+};
+enum { kCaOpen = 1, kCaClosed = 2 };     // a block begins here and is not finished; a block that began before is finished here
+
+// A sequence as the kernel takes it: what the host promised is also a bound.
+struct CaSeq {
+  int base, n_all, n, ctx, rows, blocks;
+  __device__ __forceinline__ void load(const ChunkArgs& a, int s, int rep) {
+    base = a.cu[s];
+    n_all = a.cu[s + 1] - base;
+    n = base < 0 ? 0 : max(0, min(min(n_all, a.max_new), a.T - base));
+    ctx = max(0, min(a.ctx[s], a.max_ctx));
+    rows = n * rep;
+    blocks = (rows + kCaBlock - 1) / kCaBlock;
+  }
+  __device__ __forceinline__ int block_rows(int b) const { return min(kCaBlock, rows - b * kCaBlock); }
+  __device__ __forceinline__ bool dual(int b) const { return rows - b * kCaBlock <= kCaRows; }
+  __device__ __forceinline__ int keys(int b, int rep) const {   // visible to the block's last row
+    const int token = (b * kCaBlock + block_rows(b) - 1) / rep;
+    return max(0, min(ctx, ctx - n_all + token + 1));
+  }
+  __device__ __forceinline__ int tiles(int b, int rep) const { return max(1, (keys(b, rep) + kCaKeys - 1) / kCaKeys); }
+  __device__ __forceinline__ int units(int b, int rep) const { return tiles(b, rep) * (dual(b) ? 1 : 2); }
 };
 
-// One warp per (row, query head): lanes over the head's dimensions, keys one after the other.
+struct CaPos {
+  int seq, kvh, blk, tile;
+  __device__ __forceinline__ bool same_block(const CaPos& o) const { return seq == o.seq && kvh == o.kvh && blk == o.blk; }
+};
+
+struct CaShared {
+  uint64_t q_full, q_empty, full[8], empty[8], s_full[2], p_ready[2], o_done[2], mma_done;
+  uint32_t tmem, dead;
+  CaPos begin, end;
+  float2 other[kCaRows];   // maximum and sum of the second stream's rows
+};
+
 template <int D>
-__global__ void __launch_bounds__(128) chunk_attn_rows_kernel(const ChunkArgs a) {
-  constexpr int E = D / 32;
-  const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int first = max(0, a.cu[s]), n = a.cu[s + 1] - a.cu[s];
-  if (i >= n || i >= a.max_new || first + i >= a.T) return;
-  const int end = min(min(a.ctx[s], a.max_ctx), a.max_pages * a.page_size) - n + i + 1;
-  const bf16* q = a.q + (long long)(first + i) * a.ldq + h * D + lane * E;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
+struct CaShape {
+  static constexpr int kBoxes = D / 64, kTile = kBoxes * kCaBox, kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSmem = (2 + kSlots) * kTile + (int)sizeof(CaShared);
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+};
+
+// ---------------------------------------------------------------------------------------------------- the line of work and its parts
+__device__ __forceinline__ long long ca_warp_sum(long long v) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) qv[e] = __bfloat162float(q[e]) * a.scale_log2, o[e] = 0.f;
-  const int g = h / (a.Hq / a.Hkv);
-  for (int j = 0; j < end; ++j) {
-    const int page = a.table[(long long)s * a.max_pages + j / a.page_size];
-    const bool there = page >= 0 && page < a.n_pages;
-    const bf16* k = a.pool + (((long long)(there ? page : 0) * 2 * a.Hkv + g) * a.page_size + j % a.page_size) * D + lane * E;
-    const bf16* v = k + (long long)a.Hkv * a.page_size * D;
-    float dot = 0.f;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long ca_warp_scan(long long v, int lane) {   // inclusive
 #pragma unroll
-    for (int e = 0; e < E; ++e) dot += qv[e] * (there ? __bfloat162float(k[e]) : 0.f);
-    dot = warp_sum(dot);
-    const float top = fmaxf(m, dot), f = exp2f(m - top), p = exp2f(dot - top);
-    l = l * f + p;
-    m = top;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * (there ? __bfloat162float(v[e]) : 0.f);
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
   }
-  bf16* out = a.out + (long long)(first + i) * a.ldo + h * D + lane * E;
+  return v;
+}
+__device__ __forceinline__ CaSeq ca_shfl(const CaSeq& q, int from) {
+  CaSeq r;
+  r.base = 0;
+  r.n_all = __shfl_sync(0xffffffffu, q.n_all, from);
+  r.n = __shfl_sync(0xffffffffu, q.n, from);
+  r.ctx = __shfl_sync(0xffffffffu, q.ctx, from);
+  r.rows = __shfl_sync(0xffffffffu, q.rows, from);
+  r.blocks = __shfl_sync(0xffffffffu, q.blocks, from);
+  return r;
+}
+// Units of the lane's sequence for one key/value head. All lanes together.
+__device__ __forceinline__ long long ca_units(const CaSeq& q, int rep, int lane) {
+  long long mine = q.blocks == 1 ? q.units(0, rep) : 0;
+  for (unsigned int many = __ballot_sync(0xffffffffu, q.blocks > 1); many != 0; many &= many - 1) {
+    const int from = __ffs(many) - 1;
+    const CaSeq w = ca_shfl(q, from);
+    long long sum = 0;
+    for (int b = lane; b < w.blocks; b += 32) sum += w.units(b, rep);
+    sum = ca_warp_sum(sum);
+    if (lane == from) mine = sum;
+  }
+  return mine;
+}
+__device__ __forceinline__ CaSeq ca_lane_seq(const ChunkArgs& a, int s, int rep) {
+  CaSeq q{0, 0, 0, 0, 0, 0};
+  if (s < a.n_seq) q.load(a, s, rep);
+  return q;
+}
+// Where unit u of the line lies; a position behind the last sequence for u = total. A warp together.
+__device__ CaPos ca_locate(const ChunkArgs& a, long long u, int rep, int lane) {
+  long long before = 0;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+    const CaSeq q = ca_lane_seq(a, s0 + lane, rep);
+    const long long one = ca_units(q, rep, lane), upto = before + ca_warp_scan(one * a.Hkv, lane);
+    const unsigned int hit = __ballot_sync(0xffffffffu, u < upto);
+    before = __shfl_sync(0xffffffffu, upto, 31);
+    if (hit == 0) continue;
+    const int from = __ffs(hit) - 1;
+    const long long per = __shfl_sync(0xffffffffu, one, from), start = __shfl_sync(0xffffffffu, upto, from) - per * a.Hkv;
+    const CaSeq w = ca_shfl(q, from);
+    CaPos p;
+    p.seq = s0 + from;
+    p.kvh = (int)((u - start) / per);
+    long long rest = (u - start) - p.kvh * per;
+    p.blk = 0;
+    for (int b0 = 0; b0 < w.blocks; b0 += 32) {
+      const int b = b0 + lane;
+      const long long up = ca_warp_scan(b < w.blocks ? w.units(b, rep) : 0, lane), all = __shfl_sync(0xffffffffu, up, 31);
+      const unsigned int in = __ballot_sync(0xffffffffu, rest < up);
+      if (in != 0) {
+        const int l = __ffs(in) - 1;
+        const long long low = __shfl_sync(0xffffffffu, up, l > 0 ? l - 1 : 0);
+        p.blk = b0 + l;
+        rest -= l > 0 ? low : 0;
+        break;
+      }
+      rest -= all;
+    }
+    p.tile = w.dual(p.blk) ? (int)rest : (int)(rest >> 1);
+    return p;
+  }
+  return CaPos{a.n_seq, 0, 0, 0};
+}
+// The CTA's part [begin, end) of the line, and what it says about the blocks that are cut. Warp 0.
+__device__ void ca_span(const ChunkArgs& a, CaShared* sh, int rep, int lane) {
+  long long total = 0;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 32) total += ca_units(ca_lane_seq(a, s0 + lane, rep), rep, lane);
+  total = ca_warp_sum(total) * a.Hkv;
+  const long long parts = min((long long)gridDim.x, max(1ll, total / kCaMinUnits)), cta = blockIdx.x;
+  CaPos begin{a.n_seq, 0, 0, 0}, end = begin;
+  if (cta < parts) {
+    begin = ca_locate(a, total * cta / parts, rep, lane);
+    end = ca_locate(a, total * (cta + 1) / parts, rep, lane);
+  }
+  if (lane == 0) {
+    sh->begin = begin;
+    sh->end = end;
+    if (a.head != nullptr) {
+      int4 head = make_int4(0, 0, 0, 0);
+      const bool one = begin.same_block(end);
+      if (begin.tile > 0 && !one) head.x |= kCaClosed;
+      if (end.tile > 0 && (!one || begin.tile == 0)) {
+        CaSeq q;
+        q.load(a, end.seq, rep);
+        head.x |= kCaOpen;
+        head.y = q.base;
+        head.z = end.blk * kCaBlock;
+        head.w = q.block_rows(end.blk) | end.kvh << 16;
+      }
+      a.head[cta] = head;
+    }
+  }
+}
+
+// The blocks of a CTA's part one after the other; every warp walks for itself.
+struct CaWalk {
+  CaPos at;
+  CaSeq q;
+  int t0, t1, tiles, keys, row0, n_rows;
+  bool dual, last;
+  __device__ __forceinline__ bool enter(const ChunkArgs& a, const CaShared* sh, int rep) {
+    if (at.seq >= a.n_seq) return false;
+    last = at.same_block(sh->end);
+    if (last && sh->end.tile <= at.tile) return false;
+    row0 = at.blk * kCaBlock;
+    n_rows = q.block_rows(at.blk);
+    dual = q.dual(at.blk);
+    keys = q.keys(at.blk, rep);
+    tiles = max(1, (keys + kCaKeys - 1) / kCaKeys);
+    t0 = at.tile;
+    t1 = last ? sh->end.tile : tiles;
+    return true;
+  }
+  __device__ __forceinline__ bool first(const ChunkArgs& a, const CaShared* sh, int rep) {
+    at = sh->begin;
+    if (at.seq < a.n_seq) q.load(a, at.seq, rep);
+    return enter(a, sh, rep);
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs& a, const CaShared* sh, int rep) {
+    if (last) return false;
+    at.tile = 0;
+    if (++at.blk == q.blocks) {
+      at.blk = 0;
+      if (++at.kvh == a.Hkv) {
+        at.kvh = 0;
+        do {
+          if (++at.seq >= a.n_seq) return false;
+          q.load(a, at.seq, rep);
+        } while (q.blocks == 0);
+      }
+    }
+    return enter(a, sh, rep);
+  }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
+  __device__ __forceinline__ int count(int stream) const { return dual ? (t1 - t0 + 1 - stream) >> 1 : t1 - t0; }   // tiles of a stream
+  __device__ __forceinline__ int tile(int stream, int j) const { return dual ? 2 * j + stream : j; }                // its j-th, from t0 on
+};
+
+// ---------------------------------------------------------------------------------------------------- small pieces
+__device__ __forceinline__ bool ca_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+template <int R>
+__device__ __forceinline__ void ca_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void ca_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int ID>
+__device__ __forceinline__ void ca_streams_sync() { asm volatile("bar.sync %0, 256;" ::"n"(ID) : "memory"); }   // the 256 threads of both streams
+__device__ __forceinline__ float ca_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The maximum keeps a NaN: it then is the row's reference, and the row becomes NaN whichever unit its exponentials come from.
+__device__ __forceinline__ float ca_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t ca_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void ca_f2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t ca_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t ca_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x of two numbers on the multiply-add pipe: n = round(x) by adding 1.5 2^23, 2^(x - n) on [-1/2, 1/2] by its Taylor polynomial of degree 4 with the last
+// coefficients fitted (4e-5), n added to the exponent.
+__device__ __forceinline__ void ca_ex2_fma(float x0, float x1, float& e0, float& e1) {
+  const uint64_t x = ca_f2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = ca_add2(x, ca_f2(12582912.f, 12582912.f));
+  const uint64_t f = ca_fma2(ca_add2(t, ca_f2(-12582912.f, -12582912.f)), ca_f2(-1.f, -1.f), x);
+  uint64_t p = ca_fma2(ca_f2(0.00961812911f, 0.00961812911f), f, ca_f2(0.0555041087f, 0.0555041087f));
+  p = ca_fma2(p, f, ca_f2(0.240226507f, 0.240226507f));
+  p = ca_fma2(p, f, ca_f2(0.693147181f, 0.693147181f));
+  p = ca_fma2(p, f, ca_f2(1.f, 1.f));
+  float t0, t1, p0, p1;
+  ca_f2(t, t0, t1);
+  ca_f2(p, p0, p1);
+  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// ---------------------------------------------------------------------------------------------------- the kernel
+template <int D>
+__global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkArgs a) {
+  using C = CaShape<D>;
+  extern __shared__ __align__(1024) uint8_t ca_smem[];
+  uint8_t* const qs = ca_smem;                           // [2 tiles][box][128 rows][128 B]
+  uint8_t* const ring = qs + 2 * C::kTile;               // [slot][box][128 keys][128 B]: keys, values, keys, ...
+  CaShared* const sh = reinterpret_cast<CaShared*>(ring + C::kSlots * C::kTile);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rep = a.Hq / a.Hkv;
+  pdl_launch();
+  const WaitReport report{&sh->dead, &g_chunk_failures, a.failed};
+  if (warp == 0) ca_span(a, sh, rep, lane);
+  if (warp == 12) {
+    if (elect_one()) {
+      mbar_init(&sh->q_full, 3);
+      mbar_init(&sh->q_empty, 1);
+      for (int i = 0; i < C::kSlots; ++i) {
+        mbar_init(&sh->full[i], 4);
+        mbar_init(&sh->empty[i], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&sh->s_full[t], 1);
+        mbar_init(&sh->p_ready[t], 4);
+        mbar_init(&sh->o_done[t], 1);
+      }
+      mbar_init(&sh->mma_done, 1);
+      sh->dead = 0u;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc<1>(&sh->tmem, 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;                        // S of stream t at 128 t (P over its first 64 columns), O at 256 + 128 t
+  CaWalk w;
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------------------------------ keys and values
+    ca_regs_down<kCaRegsLoad>();
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes;    // lanes of a row, rows of a warp at a time
+    const int c = lane % kLanes, sub = lane / kLanes;
+    int copy = 0, told = 0, slot = 0, told_slot = 0;
+    uint32_t parity = 1;
+    auto tell = [&]() {                                  // copy `told` is there, and visible to the products
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->full[told_slot]);
+      ++told;
+      if (++told_slot == C::kSlots) told_slot = 0;
+    };
+    bool go = true;
+    for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep)) {
+      const int32_t* bt = a.table + (long long)w.at.seq * a.max_pages;
+      for (int tile = w.t0; go && tile < w.t1; ++tile) {
+        const int key = tile * kCaKeys + warp * 32 + lane;
+        int row = -1;                                    // of the pool, in rows of D
+        if (key < w.keys) {
+          const int index = key / a.page_size, page = bt[index];
+          if (page >= 0 && page < a.n_pages) row = (page * 2 * a.Hkv + w.at.kvh) * a.page_size + key - index * a.page_size;
+        }
+#pragma unroll 1
+        for (int values = 0; values < 2; ++values) {
+          if (!__all_sync(0xffffffffu, ca_test(&sh->empty[slot], parity))) {
+            // no room: what is under way is told of first, the products may wait for it
+            if (told < copy) cp_async_wait<0>();
+            while (told < copy) tell();
+            if (!wait_bounded_warp(&sh->empty[slot], parity, report)) {
+              go = false;
+              break;
+            }
+          }
+          uint8_t* dst = ring + slot * C::kTile + (c >> 3) * kCaBox + warp * 32 * 128;
+          const int from = row < 0 ? -1 : row + values * a.Hkv * a.page_size;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = __float2bfloat16(l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l));
+          for (int i = 0; i < 32 / kPer; ++i) {
+            const int r = i * kPer + sub, at = __shfl_sync(0xffffffffu, from, r);
+            cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), a.pool + (long long)max(at, 0) * D + c * 8, at >= 0);
+          }
+          cp_async_commit();
+          ++copy;
+          if (++slot == C::kSlots) {
+            slot = 0;
+            parity ^= 1u;
+          }
+          if (copy - told > 2) {
+            cp_async_wait<2>();
+            tell();
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    while (go && told < copy) tell();
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------------------------------ softmax and epilogue
+    ca_regs_up<kCaRegsSoftmax>();
+    const int t = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + lanes + (uint32_t)(t * 128), to = tmem + lanes + 256u;
+    const float sl2 = a.scale_log2, grown = 8.f / sl2;
+    // the lanes of a warp may leave a wait one by one, and accesses to tensor memory are the warp's as a whole; whether the phase came is not asked
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      wait_bounded(bar, parity, report);
+      __syncwarp();
+    };
+    uint32_t done = 0;                                   // tiles of this stream so far
+    for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep)) {
+      const int mine = w.count(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
+      const bool any = row - lane < w.n_rows, is_row = row < w.n_rows;
+      const int token = (w.row0 + row) / rep, h = w.row0 + row - token * rep, p = w.q.ctx - w.q.n_all + token;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < mine; ++j, ++done) {
+        wait(&sh->s_full[t], done & 1u);
+        tc_fence_after();
+        if (any) {
+          uint32_t v[kCaKeys];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32u * i, v + 32 * i);
+          tmem_ld_wait();
+          const int lim = p - (w.t0 + w.tile(t, j)) * kCaKeys;   // the tile's last visible key
+          const bool masked = !__all_sync(0xffffffffu, lim >= kCaKeys - 1);
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < kCaKeys; ++i) v[i] = i <= lim ? v[i] : 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kCaKeys; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = ca_max3(mx[e], __uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
+          }
+          const float top = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+          // the reference moves only when the maximum grew by more than 2^8: sums and products are exact in it, and O is seldom touched
+          const bool grow = is_row && !(top <= m + grown);   // rows behind the block's last hold whatever lay in shared memory
+          const bool rescale = __any_sync(0xffffffffu, grow);
+          float f = 1.f;
+          if (grow) {
+            f = ca_ex2((m - top) * sl2);
+            l *= f;
+            m = top;
+          }
+          const float neg = m == -INFINITY ? 0.f : -m * sl2;
+          const uint64_t sl2_2 = ca_f2(sl2, sl2), neg_2 = ca_f2(neg, neg);
+          uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int at = b * 32 + 2 * i;
+              float x0, x1, e0, e1;
+              ca_f2(ca_fma2(ca_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl2_2, neg_2), x0, x1);
+              // three of eight pairs leave the exponential unit (16 a cycle) to the others; hidden scores have to become zeros exactly
+              if (!masked && (0x52 >> (i & 7) & 1)) ca_ex2_fma(x0, x1, e0, e1);
+              else e0 = ca_ex2(x0), e1 = ca_ex2(x1);
+              sum[i & 3] = ca_add2(sum[i & 3], ca_f2(e0, e1));
+              pk[i] = pack_bf16(e0, e1);
+            }
+            tmem_st16(ts + 16u * b, pk);
+          }
+          float s0, s1;
+          ca_f2(ca_add2(ca_add2(sum[0], sum[1]), ca_add2(sum[2], sum[3])), s0, s1);
+          l += s0 + s1;
+          if (rescale && j > 0) {                        // the scores were there, so the output product in front of them is done
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + (uint32_t)(t * 128 + c0), o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(to + (uint32_t)(t * 128 + c0), o);
+            }
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_ready[t]);
+      }
+      if (mine > 0) wait(&sh->o_done[t], (done - 1u) & 1u);
+      tc_fence_after();
+      float own_f = 1.f, other_f = 0.f, m2 = m * sl2;    // m2: in base 2
+      bool two = false;
+      if (w.dual) {
+        if (t == 1) sh->other[lane_row] = make_float2(m2, l);
+        tc_fence_before();
+        ca_streams_sync<1>();
+        tc_fence_after();
+        if (t == 0) {
+          const float2 o = sh->other[lane_row];
+          two = w.count(1) > 0;
+          const float top = ca_max3(m2, o.x, o.x);
+          own_f = m2 == -INFINITY ? 0.f : ca_ex2(m2 - top);
+          other_f = o.x == -INFINITY ? 0.f : ca_ex2(o.x - top);
+          l = l * own_f + o.y * other_f;
+          m2 = top;
+        }
+      }
+      if (any && !(w.dual && t == 1)) {
+        const bool whole = w.whole();
+        const long long part = 2ll * blockIdx.x + (w.t0 > 0 ? 0 : 1);
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f, f0 = own_f * inv, f1 = other_f * inv;
+        bf16* const orow = a.out + (long long)(w.q.base + token) * a.ldo + (long long)(w.at.kvh * rep + h) * D;
+        float* const prow = a.part + (part * a.part_rows + row) * D;
+        if (!whole && is_row) a.ml[part * a.part_rows + row] = make_float2(m2, l);
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld32(to + (uint32_t)((w.dual ? 0 : t * 128) + c0), v);
+          tmem_ld_wait();
+          float o[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f0 == 0.f ? 0.f : __uint_as_float(v[i]) * f0;
+          if (two) {
+            tmem_ld32(to + (uint32_t)(128 + c0), v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] += f1 == 0.f ? 0.f : __uint_as_float(v[i]) * f1;
+          }
+          if (is_row) {
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) dst[i / 8] = make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]), pack_bf16(o[i + 6], o[i + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(prow + c0);
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+          __syncwarp();                                  // the next load of tensor memory wants the whole warp
+        }
+      }
+      tc_fence_before();
+      if (w.dual) ca_streams_sync<2>();                  // the second stream's O and sums have been read
+    }
+  } else {
+    ca_regs_down<kCaRegsIssue>();
+    if (warp == 12) {
+      // ---------------------------------------------------------------------------------------- products
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = make_idesc_bf16_major(kCaRows, kCaKeys, 0, 0), idesc_o = make_idesc_bf16_major(kCaRows, D, 0, 1);
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bounded(bar, parity, report); };
+        uint32_t pv[2] = {0, 0}, seg = 0;                // output products issued per stream, blocks
+        int copy = 0;                                    // of the block's first keys
+        bool go = true;
+        for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep), ++seg) {
+          const int n[2] = {w.count(0), w.count(1)};
+          int left = n[0] + n[1];
+          auto arrived = [&](int i) { return wait(&sh->full[i % C::kSlots], (uint32_t)(i / C::kSlots) & 1u); };
+          auto scores = [&](int t, int j) {
+            const int i = copy + 2 * w.tile(t, j);
+            if ((w.dual || t == 0) && !arrived(i)) return false;
+            // over the probabilities of the tile before: the order of products is only promised for one accumulator, so the one that reads them has to
+            // be done, not only issued
+            if (pv[t] > 0 && !wait(&sh->o_done[t], (pv[t] - 1u) & 1u)) return false;
+            tc_fence_after();
+            const uint32_t q0 = smem_u32(qs + (w.dual ? 0 : t * C::kTile)), k0 = smem_u32(ring + i % C::kSlots * C::kTile);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16<1>(tmem + (uint32_t)(t * 128), make_sw128_kmajor_desc(q0 + (k >> 2) * kCaBox) + (uint64_t)(2 * (k & 3)),
+                           make_sw128_kmajor_desc(k0 + (k >> 2) * kCaBox) + (uint64_t)(2 * (k & 3)), idesc_s, k != 0 ? 1u : 0u);
+            umma_commit(&sh->s_full[t]);
+            if (w.dual || t == 1) umma_commit(&sh->empty[i % C::kSlots]);
+            if (--left == 0) umma_commit(&sh->q_empty);
+            return true;
+          };
+          go = wait(&sh->q_full, seg & 1u);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (go && n[t] > 0) go = scores(t, 0);
+          for (int j = 0; go && j < n[0]; ++j) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!go || j >= n[t]) continue;
+              const int i = copy + 2 * w.tile(t, j) + 1;
+              go = wait(&sh->p_ready[t], pv[t] & 1u) && (!(w.dual || t == 0) || arrived(i));
+              if (!go) continue;
+              tc_fence_after();
+              const uint32_t v0 = smem_u32(ring + i % C::kSlots * C::kTile);
+#pragma unroll
+              for (int k = 0; k < kCaKeys / 16; ++k)
+                umma_bf16_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * 128 + 8 * k), make_sw128_mnmajor_desc(v0 + k * 2048, kCaBox, 1024), idesc_o, (j | k) != 0 ? 1u : 0u);
+              umma_commit(&sh->o_done[t]);
+              ++pv[t];
+              if (w.dual || t == 1) umma_commit(&sh->empty[i % C::kSlots]);
+              if (j + 1 < n[t]) go = scores(t, j + 1);
+            }
+          }
+          copy += 2 * (w.t1 - w.t0);
+        }
+        umma_commit(&sh->mma_done);
+        drain_bounded(&sh->mma_done, 0, report);         // every product that was issued is done
+      }
+    } else {
+      // ---------------------------------------------------------------------------------------- queries
+      constexpr int kLanes = D / 8, kAt = 96 / kLanes;
+      const int c = (tid - 416) % kLanes, r0 = (tid - 416) / kLanes;
+      uint32_t seg = 0;
+      for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep), ++seg) {
+        if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report)) break;
+        for (int r = r0; r < w.n_rows; r += kAt) {
+          const int token = (w.row0 + r) / rep, h = w.row0 + r - token * rep;
+          const bf16* src = a.q + (long long)(w.q.base + token) * a.ldq + (long long)(w.at.kvh * rep + h) * D + c * 8;
+          cp_async16(qs + (r >> 7) * C::kTile + (c >> 3) * kCaBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, true);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->q_full);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// The parts of a block that was cut: it begins in CTA i (its second part), goes on in the CTAs behind it (their first parts) up to the one that says so. A warp
+// per row.
+template <int D>
+__global__ void __launch_bounds__(32 * kCaJoinRows) chunk_attn_join_kernel(const ChunkArgs a) {
+  pdl_wait();
+  constexpr int E = D / 32;
+  const int i = blockIdx.x, n = gridDim.x, lane = threadIdx.x & 31, row = blockIdx.y * kCaJoinRows + (threadIdx.x >> 5), rep = a.Hq / a.Hkv;
+  const int4 head = a.head[i];
+  if (!(head.x & kCaOpen) || row >= (head.w & 0xffff)) return;
+  int parts = 0;                                         // behind the first
+  for (int j0 = i + 1; j0 < n; j0 += 32) {
+    const unsigned int closed = __ballot_sync(0xffffffffu, j0 + lane < n && (a.head[min(j0 + lane, n - 1)].x & kCaClosed));
+    if (closed != 0) {
+      parts = j0 - i + __ffs(closed) - 1;
+      break;
+    }
+  }
+  auto at = [&](int k) { return (2ll * (i + k) + (k == 0 ? 1 : 0)) * a.part_rows + row; };
+  float top = -INFINITY;
+  for (int k = lane; k <= parts; k += 32) top = ca_max3(top, a.ml[at(k)].x, -INFINITY);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = ca_max3(top, __shfl_xor_sync(0xffffffffu, top, o), -INFINITY);
+  float l = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int k0 = 0; k0 <= parts; k0 += 32) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (k0 + lane <= parts) mine = a.ml[at(k0 + lane)];
+    const float f = mine.x == -INFINITY ? 0.f : ca_ex2(mine.x - top);
+    l += f * mine.y;
+    const int here = min(32, parts + 1 - k0);
+#pragma unroll 4
+    for (int k = 0; k < here; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      const float* o = a.part + at(k0 + k) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += fk == 0.f ? 0.f : o[e] * fk;   // a part in which the row saw no key
+    }
+  }
+  l = warp_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int token = (head.z + row) / rep, h = head.z + row - token * rep;
+  bf16* out = a.out + (long long)(head.y + token) * a.ldo + (long long)((head.w >> 16) * rep + h) * D + lane * E;
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+  else *reinterpret_cast<uint32_t*>(out) = pack_bf16(acc[0] * inv, acc[1] * inv);
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+struct CaPlan {
+  int grid, part_rows;
+  bool cut;                // whether a block can be cut
+  long long bytes;
+};
+static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
+  const long long rows = (long long)max_new * (Hq / Hkv), tiles = ((long long)max_ctx + kCaKeys - 1) / kCaKeys;
+  const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * (tiles > 1 ? tiles : 1);   // products there can be
+  const long long parts = most / kCaMinUnits;
+  CaPlan p;
+  const int sms = num_sms();
+  p.grid = parts < 1 ? 1 : (parts < sms ? (int)parts : sms);
+  p.part_rows = rows < kCaBlock ? (int)rows : kCaBlock;
+  p.cut = p.grid > 1 && tiles > 1;
+  p.bytes = p.cut ? (long long)p.grid * 16 + 2ll * p.grid * p.part_rows * (8 + 4ll * head_dim) : 0;
+  return p;
+}
+
+template <int D>
+static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  const int dev = cur_device();
+  if (!done[dev]) {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D>);
+    if (e == cudaSuccess && at.numRegs * 4 < kCaRegsLoad + 2 * kCaRegsSoftmax + kCaRegsIssue)
+      return set_error(OMC_ERR_CUDA, "omc_paged_chunk_attn: built with fewer registers than its warps divide");
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, CaShape<D>::kSmem);
+    if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
+  int rc = check_launch("omc_paged_chunk_attn");
+  if (rc != OMC_OK || !plan.cut) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(plan.grid, (plan.part_rows + kCaJoinRows - 1) / kCaJoinRows);
+  cfg.blockDim = dim3(32 * kCaJoinRows);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D>, a);
+  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+  return check_launch("omc_paged_chunk_attn");
 }
 
 }  // namespace omc
 
 using namespace omc;
 
+static int ca_check(int n_seq, int T, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: heads of 64 or 128");
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Hkv >= 1 << 15)
+    return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: query heads must be a multiple of the key/value heads (at most 32767)");
+  if (n_seq < 0 || T < 0 || max_new < 0 || max_ctx < 0) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: negative size");
+  if ((long long)max_new * (Hq / Hkv) >= (1ll << 31) - kCaBlock || max_ctx > (1 << 30)) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: 2^31 rows or 2^30 positions");
+  return OMC_OK;
+}
+
 extern "C" long long omc_paged_chunk_attn_workspace_bytes(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
-  (void)n_seq; (void)max_new; (void)max_ctx; (void)Hq; (void)Hkv; (void)head_dim;
-  return 0;
+  const int rc = ca_check(n_seq, 0, max_new, max_ctx, Hq, Hkv, head_dim);
+  return rc != OMC_OK ? rc : ca_plan(n_seq, max_new, max_ctx, Hq, Hkv, head_dim).bytes;
 }
 
 extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv_pool, int n_pages, const int32_t* block_table, int max_pages, int page_size,
                                     const int32_t* cu_new, const int32_t* ctx_lens, int n_seq, int T, int max_new, int max_ctx, int Hq, int Hkv, int head_dim,
                                     float scale, void* out, long long ldo, void* workspace, long long workspace_bytes, void* stream) {
-  if (head_dim != 64 && head_dim != 128) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: heads of 64 or 128");
-  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: query heads must be a multiple of the key/value heads");
+  int rc = ca_check(n_seq, T, max_new, max_ctx, Hq, Hkv, head_dim);
+  if (rc != OMC_OK) return rc;
   if (n_pages <= 0 || max_pages <= 0 || page_size <= 0) return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: bad paging parameters");
   if ((long long)n_pages * 2 * Hkv * page_size >= (1ll << 31)) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: a pool of 2^31 rows or more");
-  if (n_seq < 0 || T < 0 || max_new < 0 || max_ctx < 0) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: negative size");
   if (!(scale > 0.f) || isinf(scale)) return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: the scale has to be a positive number");
   if (ldq % 8 != 0 || ldo % 8 != 0 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv_pool) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return set_error(OMC_ERR_ALIGN, "omc_paged_chunk_attn: q, pool and out on 16-byte boundaries, row strides multiples of 8");
@@ -82,11 +761,21 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
   if (n_seq == 0 || T == 0 || max_new == 0) return OMC_OK;
   if (q == nullptr || kv_pool == nullptr || out == nullptr || block_table == nullptr || cu_new == nullptr || ctx_lens == nullptr)
     return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: null pointer");
-  (void)workspace; (void)workspace_bytes;
-  ChunkArgs a{static_cast<const bf16*>(q), ldq, static_cast<const bf16*>(kv_pool), block_table, cu_new, ctx_lens, static_cast<bf16*>(out), ldo,
-              n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, Hq, Hkv, scale * 1.4426950408889634f};
-  const dim3 grid((max_new + 3) / 4, Hq, n_seq);
-  if (head_dim == 64) chunk_attn_rows_kernel<64><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-  else chunk_attn_rows_kernel<128><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-  return check_launch("omc_paged_chunk_attn");
+  const long long reach = (long long)max_pages * page_size;
+  const CaPlan plan = ca_plan(n_seq, max_new, max_ctx, Hq, Hkv, head_dim);
+  if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
+    return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: workspace missing, too small or not on a 16-byte boundary");
+  ChunkArgs a{};
+  a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.pool = static_cast<const bf16*>(kv_pool); a.table = block_table; a.cu = cu_new; a.ctx = ctx_lens;
+  a.out = static_cast<bf16*>(out); a.ldo = ldo; a.n_seq = n_seq; a.T = T; a.max_new = max_new; a.max_ctx = reach < max_ctx ? (int)reach : max_ctx;
+  a.n_pages = n_pages; a.max_pages = max_pages; a.page_size = page_size; a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * 1.4426950408889634f;
+  if (plan.bytes > 0) {
+    a.head = static_cast<int4*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.head + plan.grid);
+    a.part = reinterpret_cast<float*>(a.ml + 2ll * plan.grid * plan.part_rows);
+    a.part_rows = plan.part_rows;
+  }
+  rc = step_failure_word(&a.failed);
+  if (rc != OMC_OK) return rc;
+  return head_dim == 64 ? ca_launch<64>(a, plan, (cudaStream_t)stream) : ca_launch<128>(a, plan, (cudaStream_t)stream);
 }
