@@ -6,7 +6,8 @@
 // Rows are the (token, query head) pairs of one key/value head, token by token, so that a tile of keys is read once for all heads of a group and a single
 // token of 28 heads on 4 is a tile of 7 rows. A block is 256 rows of a sequence and a key/value head, a tile 128 keys.
 //   two streams of 128 rows take turns on the tensor pipe: S = Q K^T into TMEM, softmax in registers (a thread per row, running maximum and sum), P back to
-//   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. While one stream is in its softmax the pipe works for the other.
+//   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. Scores are made for 64 keys at a time, into two buffers per stream: a
+//   product is 256 to 400 cycles of the pipe and 330 more until who waits for it goes on, so the next scores are made while these are in their softmax.
 //   A block of at most 128 rows (all of a step of single tokens) gives its one tile of queries to both streams, which take every other tile of keys and are
 //   merged at the end: the rows of a stream lie on the same lanes of TMEM.
 // One CTA per SM walks over its share of the work: the products of all blocks (128 rows x 128 keys) in one line, cut into equal parts whatever the
@@ -14,8 +15,9 @@
 // most per CTA) in the workspace, and a second kernel, launched early, joins them.
 //   warps 0..3    keys and values by cp.async (rows through the page table, any page size), a ring of tiles
 //   warps 4..11   softmax and epilogue of the two streams
-//   warp 12       MMA issuer (one thread)
-//   warps 13..15  queries
+//   warps 12, 13  MMA issuers of the two streams (one thread each: a thread's waits and its products, which are taken one after the other, would hold up the
+//                 other stream's)
+//   warps 14, 15  queries
 // Keys behind a block's last are zero-filled, so what a page holds behind a context meets no product.
 #include <math.h>
 #include <stdint.h>
@@ -27,7 +29,7 @@ namespace omc {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int kCaRows = 128, kCaKeys = 128, kCaBlock = 256, kCaThreads = 512, kCaBox = 128 * 128;   // kCaBox: bytes of 64 columns x 128 rows
+constexpr int kCaRows = 128, kCaKeys = 128, kCaHalf = 64, kCaBlock = 256, kCaThreads = 512, kCaBox = 128 * 128;   // kCaBox: bytes of 64 columns x 128 rows
 constexpr int kCaMinUnits = 4;           // products (128 rows x 128 keys) a CTA has at least
 constexpr int kCaJoinRows = 8;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
@@ -80,7 +82,7 @@ struct CaPos {
 };
 
 struct CaShared {
-  uint64_t q_full, q_empty, full[8], empty[8], s_full[2], p_ready[2], o_done[2], mma_done;
+  uint64_t q_full, q_empty, full[8], empty[8], s_full[2][2], p_ready[2][2], o_done[2], mma_done;
   uint32_t tmem, dead;
   CaPos begin, end;
   float2 other[kCaRows];   // maximum and sum of the second stream's rows
@@ -242,7 +244,14 @@ struct CaWalk {
   }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
   __device__ __forceinline__ int count(int stream) const { return dual ? (t1 - t0 + 1 - stream) >> 1 : t1 - t0; }   // tiles of a stream
-  __device__ __forceinline__ int tile(int stream, int j) const { return dual ? 2 * j + stream : j; }                // its j-th, from t0 on
+  // halves of 64 keys: the block's last one may be behind all keys
+  __device__ __forceinline__ int halves(int stream) const {
+    const bool short_end = t1 == tiles && keys <= (tiles - 1) * kCaKeys + kCaHalf && (!dual || ((t1 - t0 - 1) & 1) == stream);
+    return 2 * count(stream) - (short_end ? 1 : 0);
+  }
+  __device__ __forceinline__ int first_key(int stream, int i) const {   // of the stream's i-th half
+    return (t0 + (dual ? 2 * (i >> 1) + stream : i >> 1)) * kCaKeys + (i & 1) * kCaHalf;
+  }
 };
 
 // ---------------------------------------------------------------------------------------------------- small pieces
@@ -261,8 +270,8 @@ template <int R>
 __device__ __forceinline__ void ca_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R>
 __device__ __forceinline__ void ca_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
-template <int ID>
-__device__ __forceinline__ void ca_streams_sync() { asm volatile("bar.sync %0, 256;" ::"n"(ID) : "memory"); }   // the 256 threads of both streams
+template <int N>
+__device__ __forceinline__ void ca_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 __device__ __forceinline__ float ca_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -290,21 +299,28 @@ __device__ __forceinline__ uint64_t ca_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x of two numbers on the multiply-add pipe: n = round(x) by adding 1.5 2^23, 2^(x - n) on [-1/2, 1/2] by its Taylor polynomial of degree 4 with the last
-// coefficients fitted (4e-5), n added to the exponent.
-__device__ __forceinline__ void ca_ex2_fma(float x0, float x1, float& e0, float& e1) {
-  const uint64_t x = ca_f2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t t = ca_add2(x, ca_f2(12582912.f, 12582912.f));
-  const uint64_t f = ca_fma2(ca_add2(t, ca_f2(-12582912.f, -12582912.f)), ca_f2(-1.f, -1.f), x);
-  uint64_t p = ca_fma2(ca_f2(0.00961812911f, 0.00961812911f), f, ca_f2(0.0555041087f, 0.0555041087f));
-  p = ca_fma2(p, f, ca_f2(0.240226507f, 0.240226507f));
-  p = ca_fma2(p, f, ca_f2(0.693147181f, 0.693147181f));
-  p = ca_fma2(p, f, ca_f2(1.f, 1.f));
-  float t0, t1, p0, p1;
-  ca_f2(t, t0, t1);
-  ca_f2(p, p0, p1);
-  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+// 2^(v sl2 + neg) of 64 scores of a row, rounded to bf16 into tensor memory from column ts on; their sum, before the rounding. All on the exponential unit (8
+// cycles of a scheduler per instruction): a polynomial on the other pipes for some of them takes some 20 cycles a pair and a quarter more instructions, which
+// cost more in their cache than it gives.
+__device__ __forceinline__ float ca_probabilities(const uint32_t (&v)[kCaHalf], uint32_t ts, uint64_t sl2, uint64_t neg) {
+  uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = b * 32 + 2 * i;
+      float x0, x1;
+      ca_f2(ca_fma2(ca_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl2, neg), x0, x1);
+      const float e0 = ca_ex2(x0), e1 = ca_ex2(x1);
+      sum[i & 3] = ca_add2(sum[i & 3], ca_f2(e0, e1));
+      pk[i] = pack_bf16(e0, e1);
+    }
+    tmem_st16(ts + 16u * b, pk);
+  }
+  float s0, s1;
+  ca_f2(ca_add2(ca_add2(sum[0], sum[1]), ca_add2(sum[2], sum[3])), s0, s1);
+  return s0 + s1;
 }
 
 // ---------------------------------------------------------------------------------------------------- the kernel
@@ -321,18 +337,20 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   if (warp == 0) ca_span(a, sh, rep, lane);
   if (warp == 12) {
     if (elect_one()) {
-      mbar_init(&sh->q_full, 3);
-      mbar_init(&sh->q_empty, 1);
+      mbar_init(&sh->q_full, 2);
+      mbar_init(&sh->q_empty, 2);
       for (int i = 0; i < C::kSlots; ++i) {
         mbar_init(&sh->full[i], 4);
-        mbar_init(&sh->empty[i], 1);
+        mbar_init(&sh->empty[i], 2);
       }
       for (int t = 0; t < 2; ++t) {
-        mbar_init(&sh->s_full[t], 1);
-        mbar_init(&sh->p_ready[t], 4);
+        for (int b = 0; b < 2; ++b) {
+          mbar_init(&sh->s_full[t][b], 1);
+          mbar_init(&sh->p_ready[t][b], 4);
+        }
         mbar_init(&sh->o_done[t], 1);
       }
-      mbar_init(&sh->mma_done, 1);
+      mbar_init(&sh->mma_done, 2);
       sh->dead = 0u;
       fence_barrier_init();
     }
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh->tmem;                        // S of stream t at 128 t (P over its first 64 columns), O at 256 + 128 t
+  const uint32_t tmem = sh->tmem;                        // S of stream t: two buffers of 64 columns at 128 t, P over the first 32 of each; O at 256 + 128 t
   CaWalk w;
 
   if (warp < 4) {
@@ -406,39 +424,46 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   } else if (warp < 12) {
     // ------------------------------------------------------------------------------------------ softmax and epilogue
     ca_regs_up<kCaRegsSoftmax>();
-    const int t = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + lanes + (uint32_t)(t * 128), to = tmem + lanes + 256u;
+    const int t = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;   // TMEM lanes go by warp % 4
+    const int both = 1 + quarter;                        // barrier of the two warps of the same lanes
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, to = tmem + lanes + 256u;
     const float sl2 = a.scale_log2, grown = 8.f / sl2;
     // the lanes of a warp may leave a wait one by one, and accesses to tensor memory are the warp's as a whole; whether the phase came is not asked
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       wait_bounded(bar, parity, report);
       __syncwarp();
     };
-    uint32_t done = 0;                                   // tiles of this stream so far
+    uint32_t done = 0;                                   // halves of this stream so far
+    // The output product of the half before is done. Waited for in front of every arrival that lets the next one start: a wait knows only odd from even, and
+    // who waits for these products, here and where they are issued, can be one behind but never two.
+    auto o_before = [&](int i) {
+      if (i > 0) wait(&sh->o_done[t], (done - 1u) & 1u);
+    };
     for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep)) {
-      const int mine = w.count(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
+      const int mine = w.halves(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
       const bool any = row - lane < w.n_rows, is_row = row < w.n_rows;
       const int token = (w.row0 + row) / rep, h = w.row0 + row - token * rep, p = w.q.ctx - w.q.n_all + token;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < mine; ++j, ++done) {
-        wait(&sh->s_full[t], done & 1u);
+      for (int i = 0; i < mine; ++i, ++done) {
+        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128) + (done & 1u) * kCaHalf;
+        wait(&sh->s_full[t][done & 1u], done >> 1 & 1u);
         tc_fence_after();
         if (any) {
-          uint32_t v[kCaKeys];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32u * i, v + 32 * i);
+          uint32_t v[kCaHalf];
+          tmem_ld32(ts, v);
+          tmem_ld32(ts + 32u, v + 32);
+          const int lim = p - w.first_key(t, i);         // the last visible one of these keys
+          const bool masked = !__all_sync(0xffffffffu, lim >= kCaHalf - 1);
           tmem_ld_wait();
-          const int lim = p - (w.t0 + w.tile(t, j)) * kCaKeys;   // the tile's last visible key
-          const bool masked = !__all_sync(0xffffffffu, lim >= kCaKeys - 1);
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < kCaKeys; ++i) v[i] = i <= lim ? v[i] : 0xff800000u;
+            for (int c = 0; c < kCaHalf; ++c) v[c] = c <= lim ? v[c] : 0xff800000u;
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < kCaKeys; i += 8) {
+          for (int c = 0; c < kCaHalf; c += 8) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = ca_max3(mx[e], __uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
+            for (int e = 0; e < 4; ++e) mx[e] = ca_max3(mx[e], __uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
           }
           const float top = ca_max3(ca_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
           // the reference moves only when the maximum grew by more than 2^8: sums and products are exact in it, and O is seldom touched
@@ -452,42 +477,27 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
           }
           const float neg = m == -INFINITY ? 0.f : -m * sl2;
           const uint64_t sl2_2 = ca_f2(sl2, sl2), neg_2 = ca_f2(neg, neg);
-          uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int at = b * 32 + 2 * i;
-              float x0, x1, e0, e1;
-              ca_f2(ca_fma2(ca_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl2_2, neg_2), x0, x1);
-              // three of eight pairs leave the exponential unit (16 a cycle) to the others; hidden scores have to become zeros exactly
-              if (!masked && (0x52 >> (i & 7) & 1)) ca_ex2_fma(x0, x1, e0, e1);
-              else e0 = ca_ex2(x0), e1 = ca_ex2(x1);
-              sum[i & 3] = ca_add2(sum[i & 3], ca_f2(e0, e1));
-              pk[i] = pack_bf16(e0, e1);
-            }
-            tmem_st16(ts + 16u * b, pk);
-          }
-          float s0, s1;
-          ca_f2(ca_add2(ca_add2(sum[0], sum[1]), ca_add2(sum[2], sum[3])), s0, s1);
-          l += s0 + s1;
-          if (rescale && j > 0) {                        // the scores were there, so the output product in front of them is done
+          l += ca_probabilities(v, ts, sl2_2, neg_2);
+          o_before(i);
+          if (rescale && i > 0) {
+            tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
               uint32_t o[32];
               tmem_ld32(to + (uint32_t)(t * 128 + c0), o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
               tmem_st32(to + (uint32_t)(t * 128 + c0), o);
             }
           }
           tmem_st_wait();
+        } else {
+          o_before(i);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_ready[t]);
+        if (lane == 0) mbar_arrive(&sh->p_ready[t][done & 1u]);
       }
       if (mine > 0) wait(&sh->o_done[t], (done - 1u) & 1u);
       tc_fence_after();
@@ -496,7 +506,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       if (w.dual) {
         if (t == 1) sh->other[lane_row] = make_float2(m2, l);
         tc_fence_before();
-        ca_streams_sync<1>();
+        ca_sync<64>(both);
         tc_fence_after();
         if (t == 0) {
           const float2 o = sh->other[lane_row];
@@ -544,70 +554,89 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         }
       }
       tc_fence_before();
-      if (w.dual) ca_streams_sync<2>();                  // the second stream's O and sums have been read
+      if (w.dual) ca_sync<64>(both);                    // the second stream's O and sums have been read
     }
   } else {
     ca_regs_down<kCaRegsIssue>();
-    if (warp == 12) {
+    if (warp < 14) {
       // ---------------------------------------------------------------------------------------- products
       if (elect_one()) {
-        constexpr uint32_t idesc_s = make_idesc_bf16_major(kCaRows, kCaKeys, 0, 0), idesc_o = make_idesc_bf16_major(kCaRows, D, 0, 1);
+        constexpr uint32_t idesc_s = make_idesc_bf16_major(kCaRows, kCaHalf, 0, 0), idesc_o = make_idesc_bf16_major(kCaRows, D, 0, 1);
+        const uint64_t dq0 = make_sw128_kmajor_desc(smem_u32(qs)), dk0 = make_sw128_kmajor_desc(smem_u32(ring)), dv0 = make_sw128_mnmajor_desc(smem_u32(ring), kCaBox, 1024);
         auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bounded(bar, parity, report); };
-        uint32_t pv[2] = {0, 0}, seg = 0;                // output products issued per stream, blocks
-        int copy = 0;                                    // of the block's first keys
+        struct At {                                      // a copy's place in the ring
+          int slot;
+          uint32_t parity;
+          __device__ __forceinline__ At plus(int n) const {   // n < slots
+            const bool wrap = slot + n >= C::kSlots;
+            return At{wrap ? slot + n - C::kSlots : slot + n, wrap ? parity ^ 1u : parity};
+          }
+        };
+        const int t = warp - 12;
+        const uint32_t base = tmem + (uint32_t)(t * 128);
+        uint64_t* const o_done = &sh->o_done[t];
+        uint32_t seg = 0, pv = 0;                        // blocks; output products so far
+        At copy{0, 0};                                   // of the block's first keys
         bool go = true;
         for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep), ++seg) {
-          const int n[2] = {w.count(0), w.count(1)};
-          int left = n[0] + n[1];
-          auto arrived = [&](int i) { return wait(&sh->full[i % C::kSlots], (uint32_t)(i / C::kSlots) & 1u); };
-          auto scores = [&](int t, int j) {
-            const int i = copy + 2 * w.tile(t, j);
-            if ((w.dual || t == 0) && !arrived(i)) return false;
-            // over the probabilities of the tile before: the order of products is only promised for one accumulator, so the one that reads them has to
-            // be done, not only issued
-            if (pv[t] > 0 && !wait(&sh->o_done[t], (pv[t] - 1u) & 1u)) return false;
-            tc_fence_after();
-            const uint32_t q0 = smem_u32(qs + (w.dual ? 0 : t * C::kTile)), k0 = smem_u32(ring + i % C::kSlots * C::kTile);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_bf16<1>(tmem + (uint32_t)(t * 128), make_sw128_kmajor_desc(q0 + (k >> 2) * kCaBox) + (uint64_t)(2 * (k & 3)),
-                           make_sw128_kmajor_desc(k0 + (k >> 2) * kCaBox) + (uint64_t)(2 * (k & 3)), idesc_s, k != 0 ? 1u : 0u);
-            umma_commit(&sh->s_full[t]);
-            if (w.dual || t == 1) umma_commit(&sh->empty[i % C::kSlots]);
-            if (--left == 0) umma_commit(&sh->q_empty);
-            return true;
+          const bool dual = w.dual;
+          const int n = w.halves(t), step = dual ? 4 : 2;
+          At k = dual && t == 1 ? copy.plus(2) : copy, v = k.plus(1);
+          // a tile is free when both streams are done with it: the one that has it for itself says so twice
+          auto leave = [&](const At& at) {
+            umma_commit(&sh->empty[at.slot]);
+            if (dual) umma_commit(&sh->empty[at.slot]);
           };
+          const uint64_t dq = dq0 + (uint64_t)(dual ? 0 : t * (C::kTile >> 4));
           go = wait(&sh->q_full, seg & 1u);
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (go && n[t] > 0) go = scores(t, 0);
-          for (int j = 0; go && j < n[0]; ++j) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!go || j >= n[t]) continue;
-              const int i = copy + 2 * w.tile(t, j) + 1;
-              go = wait(&sh->p_ready[t], pv[t] & 1u) && (!(w.dual || t == 0) || arrived(i));
-              if (!go) continue;
+          if (n == 0) mbar_arrive(&sh->q_empty);
+          // scores of half i, then the output product of the half before
+#pragma unroll 1
+          for (int i = 0; go && i <= n && n > 0; ++i) {
+            if (i < n) {
+              // over the probabilities of two halves ago: the order of products is only promised for one accumulator, so the one that reads them has to be
+              // done, not only issued
+              go = (pv == 0 || wait(o_done, (pv - 1u) & 1u)) && ((i & 1) != 0 || wait(&sh->full[k.slot], k.parity));
+              if (!go) break;
               tc_fence_after();
-              const uint32_t v0 = smem_u32(ring + i % C::kSlots * C::kTile);
+              const uint32_t b = (pv + (i > 0 ? 1u : 0u)) & 1u;
+              const uint64_t dk = dk0 + (uint64_t)(k.slot * (C::kTile >> 4) + (i & 1) * (kCaHalf * 128 >> 4));
 #pragma unroll
-              for (int k = 0; k < kCaKeys / 16; ++k)
-                umma_bf16_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * 128 + 8 * k), make_sw128_mnmajor_desc(v0 + k * 2048, kCaBox, 1024), idesc_o, (j | k) != 0 ? 1u : 0u);
-              umma_commit(&sh->o_done[t]);
-              ++pv[t];
-              if (w.dual || t == 1) umma_commit(&sh->empty[i % C::kSlots]);
-              if (j + 1 < n[t]) go = scores(t, j + 1);
+              for (int e = 0; e < D / 16; ++e)
+                umma_bf16<1>(base + b * kCaHalf, dq + (uint64_t)((e >> 2) * (kCaBox >> 4) + 2 * (e & 3)), dk + (uint64_t)((e >> 2) * (kCaBox >> 4) + 2 * (e & 3)), idesc_s, e != 0 ? 1u : 0u);
+              umma_commit(&sh->s_full[t][b]);
+              if ((i & 1) != 0 || i + 1 == n) {
+                leave(k);
+                k = k.plus(step);
+                if (i + 1 == n) umma_commit(&sh->q_empty);
+              }
+            }
+            if (i > 0) {
+              const int j = i - 1;
+              go = ((j & 1) != 0 || wait(&sh->full[v.slot], v.parity)) && wait(&sh->p_ready[t][pv & 1u], pv >> 1 & 1u);
+              if (!go) break;
+              tc_fence_after();
+              const uint64_t dv = dv0 + (uint64_t)(v.slot * (C::kTile >> 4) + (j & 1) * (kCaHalf * 128 >> 4));
+              const uint32_t pt = base + (pv & 1u) * kCaHalf;
+#pragma unroll
+              for (int e = 0; e < kCaHalf / 16; ++e) umma_bf16_ts(base + 256u, pt + 8u * e, dv + (uint64_t)(e * 128), idesc_o, e != 0 || j != 0 ? 1u : 0u);
+              umma_commit(o_done);
+              ++pv;
+              if ((j & 1) != 0 || i == n) {
+                leave(v);
+                v = v.plus(step);
+              }
             }
           }
-          copy += 2 * (w.t1 - w.t0);
+          for (int i = 2 * (w.t1 - w.t0); i > 0; i -= 4) copy = copy.plus(i < 4 ? i : 4);
         }
         umma_commit(&sh->mma_done);
-        drain_bounded(&sh->mma_done, 0, report);         // every product that was issued is done
+        drain_bounded(&sh->mma_done, 0, report);         // every product that was issued, by either thread, is done
       }
     } else {
       // ---------------------------------------------------------------------------------------- queries
-      constexpr int kLanes = D / 8, kAt = 96 / kLanes;
-      const int c = (tid - 416) % kLanes, r0 = (tid - 416) / kLanes;
+      constexpr int kLanes = D / 8, kAt = 64 / kLanes;
+      const int c = (tid - 448) % kLanes, r0 = (tid - 448) / kLanes;
       uint32_t seg = 0;
       for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep), ++seg) {
         if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report)) break;
