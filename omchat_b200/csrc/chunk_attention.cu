@@ -82,7 +82,7 @@ struct CaPos {
 };
 
 struct CaShared {
-  uint64_t q_full, q_empty, full[8], empty[8], s_full[2][2], p_ready[2][2], o_done[2], mma_done;
+  uint64_t q_full, q_empty, full[8], empty[8], s_full[2][2], p_ready[2][2], o_done[2][2], mma_done;
   uint32_t tmem, dead;
   CaPos begin, end;
   float2 other[kCaRows];   // maximum and sum of the second stream's rows
@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         for (int b = 0; b < 2; ++b) {
           mbar_init(&sh->s_full[t][b], 1);
           mbar_init(&sh->p_ready[t][b], 4);
+          mbar_init(&sh->o_done[t][b], 1);
         }
-        mbar_init(&sh->o_done[t], 1);
       }
       mbar_init(&sh->mma_done, 2);
       sh->dead = 0u;
@@ -434,11 +434,9 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       __syncwarp();
     };
     uint32_t done = 0;                                   // halves of this stream so far
-    // The output product of the half before is done. Waited for in front of every arrival that lets the next one start: a wait knows only odd from even, and
-    // who waits for these products, here and where they are issued, can be one behind but never two.
-    auto o_before = [&](int i) {
-      if (i > 0) wait(&sh->o_done[t], (done - 1u) & 1u);
-    };
+    // Whether the output product of half g (counted like `done`) is done. A barrier per buffer: a wait knows only odd from even, and the scores of half g + 2 are not made
+    // before that product is done.
+    auto product = [&](uint32_t g) { wait(&sh->o_done[t][g & 1u], g >> 1 & 1u); };
     for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep)) {
       const int mine = w.halves(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
       const bool any = row - lane < w.n_rows, is_row = row < w.n_rows;
@@ -478,8 +476,8 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
           const float neg = m == -INFINITY ? 0.f : -m * sl2;
           const uint64_t sl2_2 = ca_f2(sl2, sl2), neg_2 = ca_f2(neg, neg);
           l += ca_probabilities(v, ts, sl2_2, neg_2);
-          o_before(i);
           if (rescale && i > 0) {
+            product(done - 1u);
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -492,14 +490,12 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
             }
           }
           tmem_st_wait();
-        } else {
-          o_before(i);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_ready[t][done & 1u]);
       }
-      if (mine > 0) wait(&sh->o_done[t], (done - 1u) & 1u);
+      if (mine > 0) product(done - 1u);                  // and all in front of it, of the same accumulator
       tc_fence_after();
       float own_f = 1.f, other_f = 0.f, m2 = m * sl2;    // m2: in base 2
       bool two = false;
@@ -574,7 +570,6 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         };
         const int t = warp - 12;
         const uint32_t base = tmem + (uint32_t)(t * 128);
-        uint64_t* const o_done = &sh->o_done[t];
         uint32_t seg = 0, pv = 0;                        // blocks; output products so far
         At copy{0, 0};                                   // of the block's first keys
         bool go = true;
@@ -596,10 +591,10 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
             if (i < n) {
               // over the probabilities of two halves ago: the order of products is only promised for one accumulator, so the one that reads them has to be
               // done, not only issued
-              go = (pv == 0 || wait(o_done, (pv - 1u) & 1u)) && ((i & 1) != 0 || wait(&sh->full[k.slot], k.parity));
+              const uint32_t g = pv + (i > 0 ? 1u : 0u), b = g & 1u;   // the half, over all blocks
+              go = (g < 2 || wait(&sh->o_done[t][b], (g - 2u) >> 1 & 1u)) && ((i & 1) != 0 || wait(&sh->full[k.slot], k.parity));
               if (!go) break;
               tc_fence_after();
-              const uint32_t b = (pv + (i > 0 ? 1u : 0u)) & 1u;
               const uint64_t dk = dk0 + (uint64_t)(k.slot * (C::kTile >> 4) + (i & 1) * (kCaHalf * 128 >> 4));
 #pragma unroll
               for (int e = 0; e < D / 16; ++e)
@@ -620,7 +615,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
               const uint32_t pt = base + (pv & 1u) * kCaHalf;
 #pragma unroll
               for (int e = 0; e < kCaHalf / 16; ++e) umma_bf16_ts(base + 256u, pt + 8u * e, dv + (uint64_t)(e * 128), idesc_o, e != 0 || j != 0 ? 1u : 0u);
-              umma_commit(o_done);
+              umma_commit(&sh->o_done[t][pv & 1u]);
               ++pv;
               if ((j & 1) != 0 || i == n) {
                 leave(v);
