@@ -4,16 +4,16 @@
 //   o[t, h] = sum_{j <= p(t)} softmax_j(scale q[t, h] . k[j, g]) v[j, g],  g = h / (Hq / Hkv)
 //
 // Rows are the (token, query head) pairs of one key/value head, token by token, so that a tile of keys is read once for all heads of a group and a single
-// token of 28 heads on 4 is a tile of 7 rows. A block is 256 rows of a sequence and a key/value head, a tile 128 keys.
+// token of 28 heads on 4 is a tile of 7 rows. A block is 256 rows of a sequence and a key/value head, a tile 64 keys.
 //   two streams of 128 rows take turns on the tensor pipe: S = Q K^T into TMEM, softmax in registers (a thread per row, running maximum and sum), P back to
-//   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. Scores are made for 64 keys at a time, into two buffers per stream: a
+//   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. Scores go into two buffers per stream: a
 //   product is 256 to 400 cycles of the pipe and 330 more until who waits for it goes on, so the next scores are made while these are in their softmax.
 //   A block of at most 128 rows (all of a step of single tokens) gives its one tile of queries to both streams, which take every other tile of keys and are
 //   merged at the end: the rows of a stream lie on the same lanes of TMEM.
-// One CTA per SM walks over its share of the work: the products of all blocks (128 rows x 128 keys) in one line, cut into equal parts whatever the
+// One CTA per SM walks over its share of the work: the products of all blocks (128 rows x 64 keys) in one line, cut into equal parts whatever the
 // lengths are, at a tile of keys. Each CTA finds its part from cu and ctx by itself. A block that is cut leaves its parts (unnormalised O, maximum, sum; two at
 // most per CTA) in the workspace, and a second kernel, launched early, joins them.
-//   warps 0..3    keys and values by cp.async (rows through the page table, any page size), a ring of tiles
+//   warps 0..3    keys and values by cp.async (rows through the page table, any page size) into a ring of tiles, which they fill as far as there is room
 //   warps 4..11   softmax and epilogue of the two streams
 //   warps 12, 13  MMA issuers of the two streams (one thread each: a thread's waits and its products, which are taken one after the other, would hold up the
 //                 other stream's)
@@ -29,8 +29,9 @@ namespace omc {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int kCaRows = 128, kCaKeys = 128, kCaHalf = 64, kCaBlock = 256, kCaThreads = 512, kCaBox = 128 * 128;   // kCaBox: bytes of 64 columns x 128 rows
-constexpr int kCaMinUnits = 4;           // products (128 rows x 128 keys) a CTA has at least
+constexpr int kCaRows = 128, kCaKeys = 64, kCaBlock = 256, kCaThreads = 512;
+constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
+constexpr int kCaMinUnits = 8;           // products (128 rows x 64 keys) a CTA has at least
 constexpr int kCaJoinRows = 8;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
@@ -90,8 +91,8 @@ struct CaShared {
 
 template <int D>
 struct CaShape {
-  static constexpr int kBoxes = D / 64, kTile = kBoxes * kCaBox, kSlots = D == 128 ? 5 : 8;
-  static constexpr int kSmem = (2 + kSlots) * kTile + (int)sizeof(CaShared);
+  static constexpr int kBoxes = D / 64, kQTile = kBoxes * kCaQBox, kTile = kBoxes * kCaBox, kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSmem = 2 * kQTile + 2 * kSlots * kTile + (int)sizeof(CaShared);
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -244,18 +245,11 @@ struct CaWalk {
   }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
   __device__ __forceinline__ int count(int stream) const { return dual ? (t1 - t0 + 1 - stream) >> 1 : t1 - t0; }   // tiles of a stream
-  // halves of 64 keys: the block's last one may be behind all keys
-  __device__ __forceinline__ int halves(int stream) const {
-    const bool short_end = t1 == tiles && keys <= (tiles - 1) * kCaKeys + kCaHalf && (!dual || ((t1 - t0 - 1) & 1) == stream);
-    return 2 * count(stream) - (short_end ? 1 : 0);
-  }
-  __device__ __forceinline__ int first_key(int stream, int i) const {   // of the stream's i-th half
-    return (t0 + (dual ? 2 * (i >> 1) + stream : i >> 1)) * kCaKeys + (i & 1) * kCaHalf;
-  }
+  __device__ __forceinline__ int first_key(int stream, int i) const { return (t0 + (dual ? 2 * i + stream : i)) * kCaKeys; }   // of its i-th
 };
 
 // ---------------------------------------------------------------------------------------------------- small pieces
-__device__ __forceinline__ bool ca_test(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool ca_test(uint64_t* bar, uint32_t parity) {   // without waiting
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred P;\n\t"
@@ -265,6 +259,10 @@ __device__ __forceinline__ bool ca_test(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+// One arrival of the thread when all its copies so far are there (the barrier counts every thread).
+__device__ __forceinline__ void ca_copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 template <int R>
 __device__ __forceinline__ void ca_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
@@ -315,10 +313,10 @@ __device__ __forceinline__ void ca_ex2_fma(float x0, float x1, float& e0, float&
   e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
-// 2^(v sl2 + neg) of 64 scores of a row, rounded to bf16 into tensor memory from column ts on; their sum, before the rounding. Two of eight pairs leave the
+// 2^(v sl2 + neg) of a row's scores, rounded to bf16 into tensor memory from column ts on; their sum, before the rounding. Two of eight pairs leave the
 // exponential unit (8 cycles of a scheduler per instruction) to the others. Measured at 2048 rows behind 28672: none 845 us, one 828, two 815, three 827. A hidden
 // score is 2^-126 there and not zero, which changes no sum that has a visible one in it.
-__device__ __forceinline__ float ca_probabilities(const uint32_t (&v)[kCaHalf], uint32_t ts, uint64_t sl2, uint64_t neg) {
+__device__ __forceinline__ float ca_probabilities(const uint32_t (&v)[kCaKeys], uint32_t ts, uint64_t sl2, uint64_t neg) {
   uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
@@ -347,8 +345,8 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   using C = CaShape<D>;
   extern __shared__ __align__(1024) uint8_t ca_smem[];
   uint8_t* const qs = ca_smem;                           // [2 tiles][box][128 rows][128 B]
-  uint8_t* const ring = qs + 2 * C::kTile;               // [slot][box][128 keys][128 B]: keys, values, keys, ...
-  CaShared* const sh = reinterpret_cast<CaShared*>(ring + C::kSlots * C::kTile);
+  uint8_t* const ring = qs + 2 * C::kQTile;              // [slot][keys, values][box][64 keys][128 B]
+  CaShared* const sh = reinterpret_cast<CaShared*>(ring + 2 * C::kSlots * C::kTile);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rep = a.Hq / a.Hkv;
   pdl_launch();
   const WaitReport report{&sh->dead, &g_chunk_failures, a.failed};
@@ -358,7 +356,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       mbar_init(&sh->q_full, 2);
       mbar_init(&sh->q_empty, 2);
       for (int i = 0; i < C::kSlots; ++i) {
-        mbar_init(&sh->full[i], 4);
+        mbar_init(&sh->full[i], 128);
         mbar_init(&sh->empty[i], 2);
       }
       for (int t = 0; t < 2; ++t) {
@@ -385,60 +383,40 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   if (warp < 4) {
     // ------------------------------------------------------------------------------------------ keys and values
     ca_regs_down<kCaRegsLoad>();
-    constexpr int kLanes = D / 8, kPer = 32 / kLanes;    // lanes of a row, rows of a warp at a time
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes, kOwn = kCaKeys / 4;   // lanes of a row, rows of a warp at a time, rows of a warp
     const int c = lane % kLanes, sub = lane / kLanes;
-    int copy = 0, told = 0, slot = 0, told_slot = 0;
+    int slot = 0;
     uint32_t parity = 1;
-    auto tell = [&]() {                                  // copy `told` is there, and visible to the products
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->full[told_slot]);
-      ++told;
-      if (++told_slot == C::kSlots) told_slot = 0;
-    };
     bool go = true;
     for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep)) {
       const int32_t* bt = a.table + (long long)w.at.seq * a.max_pages;
       for (int tile = w.t0; go && tile < w.t1; ++tile) {
-        const int key = tile * kCaKeys + warp * 32 + lane;
+        const int key = tile * kCaKeys + warp * kOwn + lane;
         int row = -1;                                    // of the pool, in rows of D
-        if (key < w.keys) {
+        if (lane < kOwn && key < w.keys) {
           const int index = key / a.page_size, page = bt[index];
           if (page >= 0 && page < a.n_pages) row = (page * 2 * a.Hkv + w.at.kvh) * a.page_size + key - index * a.page_size;
         }
+        go = wait_bounded_warp(&sh->empty[slot], parity, report);
+        if (!go) break;
 #pragma unroll 1
         for (int values = 0; values < 2; ++values) {
-          if (!__all_sync(0xffffffffu, ca_test(&sh->empty[slot], parity))) {
-            // no room: what is under way is told of first, the products may wait for it
-            if (told < copy) cp_async_wait<0>();
-            while (told < copy) tell();
-            if (!wait_bounded_warp(&sh->empty[slot], parity, report)) {
-              go = false;
-              break;
-            }
-          }
-          uint8_t* dst = ring + slot * C::kTile + (c >> 3) * kCaBox + warp * 32 * 128;
+          uint8_t* dst = ring + (2 * slot + values) * C::kTile + (c >> 3) * kCaBox + warp * kOwn * 128;
           const int from = row < 0 ? -1 : row + values * a.Hkv * a.page_size;
 #pragma unroll
-          for (int i = 0; i < 32 / kPer; ++i) {
+          for (int i = 0; i < kOwn / kPer; ++i) {
             const int r = i * kPer + sub, at = __shfl_sync(0xffffffffu, from, r);
             cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), a.pool + (long long)max(at, 0) * D + c * 8, at >= 0);
           }
-          cp_async_commit();
-          ++copy;
-          if (++slot == C::kSlots) {
-            slot = 0;
-            parity ^= 1u;
-          }
-          if (copy - told > 2) {
-            cp_async_wait<2>();
-            tell();
-          }
+        }
+        ca_copies_arrive(&sh->full[slot]);
+        if (++slot == C::kSlots) {
+          slot = 0;
+          parity ^= 1u;
         }
       }
     }
     cp_async_wait<0>();
-    while (go && told < copy) tell();
   } else if (warp < 12) {
     // ------------------------------------------------------------------------------------------ softmax and epilogue
     ca_regs_up<kCaRegsSoftmax>();
@@ -451,33 +429,33 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       wait_bounded(bar, parity, report);
       __syncwarp();
     };
-    uint32_t done = 0;                                   // halves of this stream so far
-    // Whether the output product of half g (counted like `done`) is done. A barrier per buffer: a wait knows only odd from even, and the scores of half g + 2 are not made
+    uint32_t done = 0;                                   // tiles of this stream so far
+    // Whether the output product of tile g (counted like `done`) is done. A barrier per buffer: a wait knows only odd from even, and the scores of tile g + 2 are not made
     // before that product is done.
     auto product = [&](uint32_t g) { wait(&sh->o_done[t][g & 1u], g >> 1 & 1u); };
     for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep)) {
-      const int mine = w.halves(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
+      const int mine = w.count(t), row = (w.dual ? 0 : t * kCaRows) + lane_row;
       const bool any = row - lane < w.n_rows, is_row = row < w.n_rows;
       const int token = (w.row0 + row) / rep, h = w.row0 + row - token * rep, p = w.q.ctx - w.q.n_all + token;
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < mine; ++i, ++done) {
-        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128) + (done & 1u) * kCaHalf;
+        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128) + (done & 1u) * kCaKeys;
         wait(&sh->s_full[t][done & 1u], done >> 1 & 1u);
         tc_fence_after();
         if (any) {
-          uint32_t v[kCaHalf];
+          uint32_t v[kCaKeys];
           tmem_ld32(ts, v);
           tmem_ld32(ts + 32u, v + 32);
           const int lim = p - w.first_key(t, i);         // the last visible one of these keys
-          const bool masked = !__all_sync(0xffffffffu, lim >= kCaHalf - 1);
+          const bool masked = !__all_sync(0xffffffffu, lim >= kCaKeys - 1);
           tmem_ld_wait();
           if (masked) {
 #pragma unroll
-            for (int c = 0; c < kCaHalf; ++c) v[c] = c <= lim ? v[c] : 0xff800000u;
+            for (int c = 0; c < kCaKeys; ++c) v[c] = c <= lim ? v[c] : 0xff800000u;
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < kCaHalf; c += 8) {
+          for (int c = 0; c < kCaKeys; c += 8) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e] = ca_max3(mx[e], __uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
           }
@@ -576,73 +554,72 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
     if (warp < 14) {
       // ---------------------------------------------------------------------------------------- products
       if (elect_one()) {
-        constexpr uint32_t idesc_s = make_idesc_bf16_major(kCaRows, kCaHalf, 0, 0), idesc_o = make_idesc_bf16_major(kCaRows, D, 0, 1);
-        const uint64_t dq0 = make_sw128_kmajor_desc(smem_u32(qs)), dk0 = make_sw128_kmajor_desc(smem_u32(ring)), dv0 = make_sw128_mnmajor_desc(smem_u32(ring), kCaBox, 1024);
+        constexpr uint32_t idesc_s = make_idesc_bf16_major(kCaRows, kCaKeys, 0, 0), idesc_o = make_idesc_bf16_major(kCaRows, D, 0, 1);
+        const uint64_t dq0 = make_sw128_kmajor_desc(smem_u32(qs)), dk0 = make_sw128_kmajor_desc(smem_u32(ring)), dv0 = make_sw128_mnmajor_desc(smem_u32(ring + C::kTile), kCaBox, 1024);
         auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_bounded(bar, parity, report); };
-        struct At {                                      // a copy's place in the ring
-          int slot;
-          uint32_t parity;
-          __device__ __forceinline__ At plus(int n) const {   // n < slots
-            const bool wrap = slot + n >= C::kSlots;
-            return At{wrap ? slot + n - C::kSlots : slot + n, wrap ? parity ^ 1u : parity};
-          }
-        };
         const int t = warp - 12;
         const uint32_t base = tmem + (uint32_t)(t * 128);
         uint32_t seg = 0, pv = 0;                        // blocks; output products so far
-        At copy{0, 0};                                   // of the block's first keys
+        int first = 0;                                   // slot and parity of the block's first tile
+        uint32_t first_parity = 0;
         bool go = true;
         for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep), ++seg) {
           const bool dual = w.dual;
-          const int n = w.halves(t), step = dual ? 4 : 2;
-          At k = dual && t == 1 ? copy.plus(2) : copy, v = k.plus(1);
-          // a tile is free when both streams are done with it: the one that has it for itself says so twice
-          auto leave = [&](const At& at) {
-            umma_commit(&sh->empty[at.slot]);
-            if (dual) umma_commit(&sh->empty[at.slot]);
+          const int n = w.count(t);
+          const uint64_t dq = dq0 + (uint64_t)(dual ? 0 : t * (C::kQTile >> 4));
+          int slot = first, back = 0;                    // of tile i, of the tile before
+          uint32_t parity = first_parity;
+          auto advance = [&]() {
+            if (++slot == C::kSlots) {
+              slot = 0;
+              parity ^= 1u;
+            }
           };
-          const uint64_t dq = dq0 + (uint64_t)(dual ? 0 : t * (C::kTile >> 4));
+          if (dual && t == 1) advance();
           go = wait(&sh->q_full, seg & 1u);
           if (n == 0) mbar_arrive(&sh->q_empty);
-          // scores of half i, then the output product of the half before
+          bool there = false;                            // tile i
+          // scores of tile i, then the output product of the tile before
 #pragma unroll 1
           for (int i = 0; go && i <= n && n > 0; ++i) {
+            const uint32_t g = pv + (i > 0 ? 1u : 0u), b = g & 1u;   // the tile, over all blocks
             if (i < n) {
-              // over the probabilities of two halves ago: the order of products is only promised for one accumulator, so the one that reads them has to be
-              // done, not only issued
-              const uint32_t g = pv + (i > 0 ? 1u : 0u), b = g & 1u;   // the half, over all blocks
-              go = (g < 2 || wait(&sh->o_done[t][b], (g - 2u) >> 1 & 1u)) && ((i & 1) != 0 || wait(&sh->full[k.slot], k.parity));
+              // The buffer held the probabilities of two tiles ago: the order of products is only promised for one accumulator, so the one that reads them has
+              // to be done, not only issued.
+              go = (there || wait(&sh->full[slot], parity)) && (g < 2 || wait(&sh->o_done[t][b], (g - 2u) >> 1 & 1u));
               if (!go) break;
+              fence_proxy_async();                       // the copies, made by other threads, before the products that read them
               tc_fence_after();
-              const uint64_t dk = dk0 + (uint64_t)(k.slot * (C::kTile >> 4) + (i & 1) * (kCaHalf * 128 >> 4));
+              const uint64_t dk = dk0 + (uint64_t)(slot * (2 * C::kTile >> 4));
 #pragma unroll
               for (int e = 0; e < D / 16; ++e)
-                umma_bf16<1>(base + b * kCaHalf, dq + (uint64_t)((e >> 2) * (kCaBox >> 4) + 2 * (e & 3)), dk + (uint64_t)((e >> 2) * (kCaBox >> 4) + 2 * (e & 3)), idesc_s, e != 0 ? 1u : 0u);
+                umma_bf16<1>(base + b * kCaKeys, dq + (uint64_t)((e >> 2) * (kCaQBox >> 4) + 2 * (e & 3)), dk + (uint64_t)((e >> 2) * (kCaBox >> 4) + 2 * (e & 3)), idesc_s, e != 0 ? 1u : 0u);
               umma_commit(&sh->s_full[t][b]);
-              if ((i & 1) != 0 || i + 1 == n) {
-                leave(k);
-                k = k.plus(step);
-                if (i + 1 == n) umma_commit(&sh->q_empty);
-              }
+              if (i + 1 == n) umma_commit(&sh->q_empty);
             }
+            const int last = back;
+            back = slot;
+            advance();
+            if (dual) advance();
+            there = i + 1 < n && ca_test(&sh->full[slot], parity);   // asked while the probabilities are not there yet
             if (i > 0) {
-              const int j = i - 1;
-              go = ((j & 1) != 0 || wait(&sh->full[v.slot], v.parity)) && wait(&sh->p_ready[t][pv & 1u], pv >> 1 & 1u);
+              go = wait(&sh->p_ready[t][pv & 1u], pv >> 1 & 1u);
               if (!go) break;
               tc_fence_after();
-              const uint64_t dv = dv0 + (uint64_t)(v.slot * (C::kTile >> 4) + (j & 1) * (kCaHalf * 128 >> 4));
-              const uint32_t pt = base + (pv & 1u) * kCaHalf;
+              const uint64_t dv = dv0 + (uint64_t)(last * (2 * C::kTile >> 4));
+              const uint32_t pt = base + (pv & 1u) * kCaKeys;
 #pragma unroll
-              for (int e = 0; e < kCaHalf / 16; ++e) umma_bf16_ts(base + 256u, pt + 8u * e, dv + (uint64_t)(e * 128), idesc_o, e != 0 || j != 0 ? 1u : 0u);
+              for (int e = 0; e < kCaKeys / 16; ++e) umma_bf16_ts(base + 256u, pt + 8u * e, dv + (uint64_t)(e * 128), idesc_o, e != 0 || i > 1 ? 1u : 0u);
               umma_commit(&sh->o_done[t][pv & 1u]);
               ++pv;
-              if ((j & 1) != 0 || i == n) {
-                leave(v);
-                v = v.plus(step);
-              }
+              // a slot is free when both streams are done with its tile: the one that has it for itself says so twice
+              umma_commit(&sh->empty[last]);
+              if (dual) umma_commit(&sh->empty[last]);
             }
           }
-          for (int i = 2 * (w.t1 - w.t0); i > 0; i -= 4) copy = copy.plus(i < 4 ? i : 4);
+          const int passed = first + w.t1 - w.t0;
+          first = passed % C::kSlots;
+          first_parity ^= (uint32_t)(passed / C::kSlots & 1);
         }
         umma_commit(&sh->mma_done);
         drain_bounded(&sh->mma_done, 0, report);         // every product that was issued, by either thread, is done
@@ -657,7 +634,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         for (int r = r0; r < w.n_rows; r += kAt) {
           const int token = (w.row0 + r) / rep, h = w.row0 + r - token * rep;
           const bf16* src = a.q + (long long)(w.q.base + token) * a.ldq + (long long)(w.at.kvh * rep + h) * D + c * 8;
-          cp_async16(qs + (r >> 7) * C::kTile + (c >> 3) * kCaBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, true);
+          cp_async16(qs + (r >> 7) * C::kQTile + (c >> 3) * kCaQBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, true);
         }
         cp_async_commit();
         cp_async_wait<0>();
