@@ -31,8 +31,9 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int kCaRows = 128, kCaKeys = 64, kCaBlock = 256, kCaThreads = 512;
 constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
-constexpr int kCaMinUnits = 8;           // products (128 rows x 64 keys) a CTA has at least
-constexpr int kCaJoinRows = 8;
+constexpr int kCaMinUnits = 2;           // products (128 rows x 64 keys) a CTA has at least: one of each stream, some 2 us. A single token behind 1087 positions: 8 units
+                                         // 16.4 us, 2 units JOIN_US
+constexpr int kCaJoinWarps = 8, kCaJoinRows = 4;   // a warp's rows
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
 static __device__ unsigned int g_chunk_failures;   // waits that ran out
@@ -48,13 +49,12 @@ struct ChunkArgs {
   long long ldo;
   int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, Hq, Hkv;
   float scale_log2;
-  int4* head;              // workspace: [CTAs] (flags, first row of q, first row of the block, rows | key/value head << 16)
+  int4* head;              // workspace: [CTAs] (parts of the block that is cut behind this CTA or 0, first row of q, first row of the block, rows | key/value head << 16)
   float2* ml;              // [2 CTAs][part_rows] maximum (base 2, scaled) and sum
   float* part;             // [2 CTAs][part_rows][D]
   int part_rows;
   unsigned int* failed;
 };
-enum { kCaOpen = 1, kCaClosed = 2 };     // a block begins here and is not finished; a block that began before is finished here
 
 // A sequence as the kernel takes it: what the host promised is also a bound.
 struct CaSeq {
@@ -133,68 +133,75 @@ __device__ __forceinline__ long long ca_units(const CaSeq& q, int rep, int lane)
   }
   return mine;
 }
-__device__ __forceinline__ CaSeq ca_lane_seq(const ChunkArgs& a, int s, int rep) {
-  CaSeq q{0, 0, 0, 0, 0, 0};
-  if (s < a.n_seq) q.load(a, s, rep);
-  return q;
-}
-// Where unit u of the line lies; a position behind the last sequence for u = total. A warp together.
-__device__ CaPos ca_locate(const ChunkArgs& a, long long u, int rep, int lane) {
-  long long before = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-    const CaSeq q = ca_lane_seq(a, s0 + lane, rep);
-    const long long one = ca_units(q, rep, lane), upto = before + ca_warp_scan(one * a.Hkv, lane);
-    const unsigned int hit = __ballot_sync(0xffffffffu, u < upto);
-    before = __shfl_sync(0xffffffffu, upto, 31);
-    if (hit == 0) continue;
-    const int from = __ffs(hit) - 1;
-    const long long per = __shfl_sync(0xffffffffu, one, from), start = __shfl_sync(0xffffffffu, upto, from) - per * a.Hkv;
-    const CaSeq w = ca_shfl(q, from);
-    CaPos p;
-    p.seq = s0 + from;
-    p.kvh = (int)((u - start) / per);
-    long long rest = (u - start) - p.kvh * per;
-    p.blk = 0;
-    for (int b0 = 0; b0 < w.blocks; b0 += 32) {
-      const int b = b0 + lane;
-      const long long up = ca_warp_scan(b < w.blocks ? w.units(b, rep) : 0, lane), all = __shfl_sync(0xffffffffu, up, 31);
-      const unsigned int in = __ballot_sync(0xffffffffu, rest < up);
-      if (in != 0) {
-        const int l = __ffs(in) - 1;
-        const long long low = __shfl_sync(0xffffffffu, up, l > 0 ? l - 1 : 0);
-        p.blk = b0 + l;
-        rest -= l > 0 ? low : 0;
-        break;
-      }
-      rest -= all;
-    }
-    p.tile = w.dual(p.blk) ? (int)rest : (int)(rest >> 1);
-    return p;
+// 32 sequences of the line, one per lane.
+struct CaGroup {
+  CaSeq q;
+  long long one, upto;     // units for one key/value head; of the line up to and with this sequence
+  __device__ __forceinline__ long long load(const ChunkArgs& a, int s, int rep, int lane, long long before) {   // the units behind the group
+    q = CaSeq{0, 0, 0, 0, 0, 0};
+    if (s < a.n_seq) q.load(a, s, rep);
+    one = ca_units(q, rep, lane);
+    upto = before + ca_warp_scan(one * a.Hkv, lane);
+    return __shfl_sync(0xffffffffu, upto, 31);
   }
-  return CaPos{a.n_seq, 0, 0, 0};
+};
+// Where unit u of the line lies, if in this group (whose first sequence is s0), and how many units the block has from there on. A warp together.
+__device__ __forceinline__ bool ca_locate(const ChunkArgs& a, const CaGroup& group, int s0, long long u, int rep, int lane, CaPos& p, int& rest_of_block) {
+  const unsigned int hit = __ballot_sync(0xffffffffu, u < group.upto);
+  if (hit == 0) return false;
+  const int from = __ffs(hit) - 1;
+  const long long per = __shfl_sync(0xffffffffu, group.one, from), start = __shfl_sync(0xffffffffu, group.upto, from) - per * a.Hkv;
+  if (u < start) return false;                           // in a group before
+  const CaSeq w = ca_shfl(group.q, from);
+  p.seq = s0 + from;
+  p.kvh = (int)((u - start) / per);
+  long long rest = (u - start) - p.kvh * per;
+  p.blk = 0;
+  for (int b0 = 0; b0 < w.blocks; b0 += 32) {
+    const int b = b0 + lane;
+    const long long up = ca_warp_scan(b < w.blocks ? w.units(b, rep) : 0, lane), all = __shfl_sync(0xffffffffu, up, 31);
+    const unsigned int in = __ballot_sync(0xffffffffu, rest < up);
+    if (in != 0) {
+      const int l = __ffs(in) - 1;
+      const long long low = __shfl_sync(0xffffffffu, up, l > 0 ? l - 1 : 0);
+      p.blk = b0 + l;
+      rest -= l > 0 ? low : 0;
+      break;
+    }
+    rest -= all;
+  }
+  const bool dual = w.dual(p.blk);
+  p.tile = dual ? (int)rest : (int)(rest >> 1);
+  rest_of_block = w.units(p.blk, rep) - (int)rest;
+  return true;
 }
-// The CTA's part [begin, end) of the line, and what it says about the blocks that are cut. Warp 0.
-__device__ void ca_span(const ChunkArgs& a, CaShared* sh, int rep, int lane) {
+// The CTA's part [begin, end) of the line, and what the second kernel has to know of the block that is cut behind it. Warp 0.
+__device__ __forceinline__ void ca_span(const ChunkArgs& a, CaShared* sh, int rep, int lane) {
+  CaGroup group;
   long long total = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 32) total += ca_units(ca_lane_seq(a, s0 + lane, rep), rep, lane);
-  total = ca_warp_sum(total) * a.Hkv;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 32) total = group.load(a, s0 + lane, rep, lane, total);
   const long long parts = min((long long)gridDim.x, max(1ll, total / kCaMinUnits)), cta = blockIdx.x;
+  const long long u0 = total * cta / parts, u1 = total * (cta + 1) / parts;
   CaPos begin{a.n_seq, 0, 0, 0}, end = begin;
+  int rest = 0, unused;
   if (cta < parts) {
-    begin = ca_locate(a, total * cta / parts, rep, lane);
-    end = ca_locate(a, total * (cta + 1) / parts, rep, lane);
+    long long before = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+      if (a.n_seq > 32) before = group.load(a, s0 + lane, rep, lane, before);
+      ca_locate(a, group, s0, u0, rep, lane, begin, unused);
+      ca_locate(a, group, s0, u1, rep, lane, end, rest);
+    }
   }
   if (lane == 0) {
     sh->begin = begin;
     sh->end = end;
     if (a.head != nullptr) {
       int4 head = make_int4(0, 0, 0, 0);
-      const bool one = begin.same_block(end);
-      if (begin.tile > 0 && !one) head.x |= kCaClosed;
-      if (end.tile > 0 && (!one || begin.tile == 0)) {
+      if (end.tile > 0 && (!begin.same_block(end) || begin.tile == 0)) {
         CaSeq q;
         q.load(a, end.seq, rep);
-        head.x |= kCaOpen;
+        // the block's last unit is u1 + rest - 1, in the last CTA j with total j / parts < u1 + rest
+        head.x = (int)(((u1 + rest) * parts - 1) / total - cta) + 1;
         head.y = q.base;
         head.z = end.blk * kCaBlock;
         head.w = q.block_rows(end.blk) | end.kvh << 16;
@@ -653,51 +660,69 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   }
 }
 
-// The parts of a block that was cut: it begins in CTA i (its second part), goes on in the CTAs behind it (their first parts) up to the one that says so. A warp
-// per row.
+// The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A warp takes some rows, one after
+// the other; nothing but the number of parts is waited for before the loads.
 template <int D>
-__global__ void __launch_bounds__(32 * kCaJoinRows) chunk_attn_join_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(32 * kCaJoinWarps) chunk_attn_join_kernel(const ChunkArgs a) {
   pdl_wait();
   constexpr int E = D / 32;
-  const int i = blockIdx.x, n = gridDim.x, lane = threadIdx.x & 31, row = blockIdx.y * kCaJoinRows + (threadIdx.x >> 5), rep = a.Hq / a.Hkv;
+  const int i = blockIdx.x, lane = threadIdx.x & 31, rep = a.Hq / a.Hkv;
   const int4 head = a.head[i];
-  if (!(head.x & kCaOpen) || row >= (head.w & 0xffff)) return;
-  int parts = 0;                                         // behind the first
-  for (int j0 = i + 1; j0 < n; j0 += 32) {
-    const unsigned int closed = __ballot_sync(0xffffffffu, j0 + lane < n && (a.head[min(j0 + lane, n - 1)].x & kCaClosed));
-    if (closed != 0) {
-      parts = j0 - i + __ffs(closed) - 1;
-      break;
-    }
-  }
-  auto at = [&](int k) { return (2ll * (i + k) + (k == 0 ? 1 : 0)) * a.part_rows + row; };
-  float top = -INFINITY;
-  for (int k = lane; k <= parts; k += 32) top = ca_max3(top, a.ml[at(k)].x, -INFINITY);
+  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16;
+  if (parts == 0) return;
+  for (int r = 0; r < kCaJoinRows; ++r) {
+    const int row = (blockIdx.y * kCaJoinRows + r) * kCaJoinWarps + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    auto at = [&](int k) { return (2ll * (i + k) + (k == 0 ? 1 : 0)) * a.part_rows + row; };
+    float top = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = ca_max3(top, __shfl_xor_sync(0xffffffffu, top, o), -INFINITY);
-  float l = 0.f, acc[E];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float2 mine = make_float2(-INFINITY, 0.f);
+      if (k0 + lane < parts) mine = a.ml[at(k0 + lane)];
+      const int here = min(32, parts - k0);
+      float4 ahead[4];                                   // the first parts' numbers, before their factors are known
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int k0 = 0; k0 <= parts; k0 += 32) {
-    float2 mine = make_float2(-INFINITY, 0.f);
-    if (k0 + lane <= parts) mine = a.ml[at(k0 + lane)];
-    const float f = mine.x == -INFINITY ? 0.f : ca_ex2(mine.x - top);
-    l += f * mine.y;
-    const int here = min(32, parts + 1 - k0);
+      for (int k = 0; k < 4; ++k) {
+        const float* o = a.part + at(k0 + min(k, here - 1)) * D + lane * E;
+        if constexpr (E == 4) ahead[k] = *reinterpret_cast<const float4*>(o);
+        else ahead[k] = make_float4(o[0], o[1], 0.f, 0.f);
+      }
+      float most = mine.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = ca_max3(most, __shfl_xor_sync(0xffffffffu, most, o), most);
+      most = ca_max3(most, top, most);
+      const float before = top == -INFINITY ? 0.f : ca_ex2(top - most), f = mine.x == -INFINITY ? 0.f : ca_ex2(mine.x - most);
+      top = most;
+      l = l * before + f * mine.y;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = before == 0.f ? 0.f : acc[e] * before;
+      auto add = [&](int k, const float4& v) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        if (fk == 0.f) return;                           // a part in which the row saw no key
+        acc[0] += v.x * fk;
+        acc[1] += v.y * fk;
+        if constexpr (E == 4) {
+          acc[2] += v.z * fk;
+          acc[3] += v.w * fk;
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < here) add(k, ahead[k]);
 #pragma unroll 4
-    for (int k = 0; k < here; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      const float* o = a.part + at(k0 + k) * D + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += fk == 0.f ? 0.f : o[e] * fk;   // a part in which the row saw no key
+      for (int k = 4; k < here; ++k) {
+        const float* o = a.part + at(k0 + k) * D + lane * E;
+        add(k, E == 4 ? *reinterpret_cast<const float4*>(o) : make_float4(o[0], o[1], 0.f, 0.f));
+      }
     }
+    l = warp_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int token = (head.z + row) / rep, h = head.z + row - token * rep;
+    bf16* out = a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+    else *reinterpret_cast<uint32_t*>(out) = pack_bf16(acc[0] * inv, acc[1] * inv);
   }
-  l = warp_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int token = (head.z + row) / rep, h = head.z + row - token * rep;
-  bf16* out = a.out + (long long)(head.y + token) * a.ldo + (long long)((head.w >> 16) * rep + h) * D + lane * E;
-  if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-  else *reinterpret_cast<uint32_t*>(out) = pack_bf16(acc[0] * inv, acc[1] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -736,8 +761,8 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   int rc = check_launch("omc_paged_chunk_attn");
   if (rc != OMC_OK || !plan.cut) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(plan.grid, (plan.part_rows + kCaJoinRows - 1) / kCaJoinRows);
-  cfg.blockDim = dim3(32 * kCaJoinRows);
+  cfg.gridDim = dim3(plan.grid, (plan.part_rows + kCaJoinRows * kCaJoinWarps - 1) / (kCaJoinRows * kCaJoinWarps));
+  cfg.blockDim = dim3(32 * kCaJoinWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
