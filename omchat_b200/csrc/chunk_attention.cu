@@ -33,7 +33,7 @@ constexpr int kCaRows = 128, kCaKeys = 64, kCaBlock = 256, kCaThreads = 512;
 constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
 constexpr int kCaMinUnits = 2;           // products (128 rows x 64 keys) a CTA has at least: one of each stream, some 2 us. A single token behind 1087 positions: 8 units
                                          // 16.4 us, 2 units JOIN_US
-constexpr int kCaJoinWarps = 8, kCaJoinRows = 4;   // a warp's rows
+constexpr int kCaJoinThreads = 256;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
 static __device__ unsigned int g_chunk_failures;   // waits that ran out
@@ -51,7 +51,7 @@ struct ChunkArgs {
   float scale_log2;
   int4* head;              // workspace: [CTAs] (parts of the block that is cut behind this CTA or 0, first row of q, first row of the block, rows | key/value head << 16)
   float2* ml;              // [2 CTAs][part_rows] maximum (base 2, scaled) and sum
-  float* part;             // [2 CTAs][part_rows][D]
+  float4* part;            // [2 CTAs][D / 4][part_rows]: the threads of a warp have neighbouring rows
   int part_rows;
   unsigned int* failed;
 };
@@ -86,6 +86,7 @@ struct CaShared {
   uint64_t q_full, q_empty, full[8], empty[8], s_full[2][2], p_ready[2][2], o_done[2][2], mma_done;
   uint32_t tmem, dead;
   CaPos begin, end;
+  CaSeq begin_seq;
   float2 other[kCaRows];   // maximum and sum of the second stream's rows
 };
 
@@ -97,22 +98,18 @@ struct CaShape {
 };
 
 // ---------------------------------------------------------------------------------------------------- the line of work and its parts
-__device__ __forceinline__ long long ca_warp_sum(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ long long ca_warp_scan(long long v, int lane) {   // inclusive
+__device__ __forceinline__ int ca_warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+__device__ __forceinline__ int ca_warp_scan(int v, int lane) {   // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, v, o);
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   return v;
 }
 __device__ __forceinline__ CaSeq ca_shfl(const CaSeq& q, int from) {
   CaSeq r;
-  r.base = 0;
+  r.base = __shfl_sync(0xffffffffu, q.base, from);
   r.n_all = __shfl_sync(0xffffffffu, q.n_all, from);
   r.n = __shfl_sync(0xffffffffu, q.n, from);
   r.ctx = __shfl_sync(0xffffffffu, q.ctx, from);
@@ -120,95 +117,96 @@ __device__ __forceinline__ CaSeq ca_shfl(const CaSeq& q, int from) {
   r.blocks = __shfl_sync(0xffffffffu, q.blocks, from);
   return r;
 }
-// Units of the lane's sequence for one key/value head. All lanes together.
-__device__ __forceinline__ long long ca_units(const CaSeq& q, int rep, int lane) {
-  long long mine = q.blocks == 1 ? q.units(0, rep) : 0;
-  for (unsigned int many = __ballot_sync(0xffffffffu, q.blocks > 1); many != 0; many &= many - 1) {
-    const int from = __ffs(many) - 1;
-    const CaSeq w = ca_shfl(q, from);
-    long long sum = 0;
-    for (int b = lane; b < w.blocks; b += 32) sum += w.units(b, rep);
-    sum = ca_warp_sum(sum);
-    if (lane == from) mine = sum;
-  }
-  return mine;
-}
 // 32 sequences of the line, one per lane.
 struct CaGroup {
   CaSeq q;
-  long long one, upto;     // units for one key/value head; of the line up to and with this sequence
-  __device__ __forceinline__ long long load(const ChunkArgs& a, int s, int rep, int lane, long long before) {   // the units behind the group
+  int one, upto;           // units for one key/value head; of the line up to and with this sequence
+  __device__ __forceinline__ int load(const ChunkArgs& a, int s, int rep, int lane, int before) {   // the units up to the group's end
     q = CaSeq{0, 0, 0, 0, 0, 0};
     if (s < a.n_seq) q.load(a, s, rep);
-    one = ca_units(q, rep, lane);
+    one = q.blocks == 1 ? q.units(0, rep) : 0;
+    for (unsigned int many = __ballot_sync(0xffffffffu, q.blocks > 1); many != 0; many &= many - 1) {
+      const int from = __ffs(many) - 1;
+      const CaSeq w = ca_shfl(q, from);
+      int sum = 0;
+      for (int b = lane; b < w.blocks; b += 32) sum += w.units(b, rep);
+      sum = ca_warp_sum(sum);
+      if (lane == from) one = sum;
+    }
     upto = before + ca_warp_scan(one * a.Hkv, lane);
     return __shfl_sync(0xffffffffu, upto, 31);
   }
 };
-// Where unit u of the line lies, if in this group (whose first sequence is s0), and how many units the block has from there on. A warp together.
-__device__ __forceinline__ bool ca_locate(const ChunkArgs& a, const CaGroup& group, int s0, long long u, int rep, int lane, CaPos& p, int& rest_of_block) {
+struct CaPlace {
+  CaPos at;
+  CaSeq q;
+  int within, left;        // units of the block in front of the place and from it on
+};
+// Where unit u of the line lies, if in this group (whose first sequence is s0). A warp together.
+__device__ __forceinline__ void ca_locate(const ChunkArgs& a, const CaGroup& group, int s0, int u, int rep, int lane, CaPlace& p) {
   const unsigned int hit = __ballot_sync(0xffffffffu, u < group.upto);
-  if (hit == 0) return false;
-  const int from = __ffs(hit) - 1;
-  const long long per = __shfl_sync(0xffffffffu, group.one, from), start = __shfl_sync(0xffffffffu, group.upto, from) - per * a.Hkv;
-  if (u < start) return false;                           // in a group before
-  const CaSeq w = ca_shfl(group.q, from);
-  p.seq = s0 + from;
-  p.kvh = (int)((u - start) / per);
-  long long rest = (u - start) - p.kvh * per;
-  p.blk = 0;
-  for (int b0 = 0; b0 < w.blocks; b0 += 32) {
-    const int b = b0 + lane;
-    const long long up = ca_warp_scan(b < w.blocks ? w.units(b, rep) : 0, lane), all = __shfl_sync(0xffffffffu, up, 31);
-    const unsigned int in = __ballot_sync(0xffffffffu, rest < up);
+  if (hit == 0) return;
+  const int from = __ffs(hit) - 1, per = __shfl_sync(0xffffffffu, group.one, from), start = __shfl_sync(0xffffffffu, group.upto, from) - per * a.Hkv;
+  if (u < start) return;                                 // in a group before
+  p.q = ca_shfl(group.q, from);
+  p.at.seq = s0 + from;
+  p.at.kvh = (u - start) / per;
+  p.within = u - start - p.at.kvh * per;
+  p.at.blk = 0;
+  for (int b0 = 0; b0 < p.q.blocks; b0 += 32) {
+    const int b = b0 + lane, mine = b < p.q.blocks ? p.q.units(b, rep) : 0, up = ca_warp_scan(mine, lane);
+    const unsigned int in = __ballot_sync(0xffffffffu, p.within < up);
     if (in != 0) {
-      const int l = __ffs(in) - 1;
-      const long long low = __shfl_sync(0xffffffffu, up, l > 0 ? l - 1 : 0);
-      p.blk = b0 + l;
-      rest -= l > 0 ? low : 0;
+      const int l = __ffs(in) - 1, all = __shfl_sync(0xffffffffu, up, l), own = __shfl_sync(0xffffffffu, mine, l);
+      p.at.blk = b0 + l;
+      p.within -= all - own;
+      p.left = own - p.within;
       break;
     }
-    rest -= all;
+    p.within -= __shfl_sync(0xffffffffu, up, 31);
   }
-  const bool dual = w.dual(p.blk);
-  p.tile = dual ? (int)rest : (int)(rest >> 1);
-  rest_of_block = w.units(p.blk, rep) - (int)rest;
-  return true;
+  p.at.tile = p.q.dual(p.at.blk) ? p.within : p.within >> 1;
 }
-// The CTA's part [begin, end) of the line, and what the second kernel has to know of the block that is cut behind it. Warp 0.
-__device__ __forceinline__ void ca_span(const ChunkArgs& a, CaShared* sh, int rep, int lane) {
+// The CTA's part [begin, end) of the line: warp 0 finds where it begins, warp 1 where it ends and what the second kernel has to know of the block that is cut there.
+__device__ __forceinline__ void ca_span(const ChunkArgs& a, CaShared* sh, int rep, int lane, bool ends) {
   CaGroup group;
-  long long total = 0;
+  int total = 0;
   for (int s0 = 0; s0 < a.n_seq; s0 += 32) total = group.load(a, s0 + lane, rep, lane, total);
-  const long long parts = min((long long)gridDim.x, max(1ll, total / kCaMinUnits)), cta = blockIdx.x;
-  const long long u0 = total * cta / parts, u1 = total * (cta + 1) / parts;
-  CaPos begin{a.n_seq, 0, 0, 0}, end = begin;
-  int rest = 0, unused;
+  const int parts = min((int)gridDim.x, max(1, total / kCaMinUnits)), cta = blockIdx.x, each = total / parts, more = total - each * parts;
+  auto cut = [&](int c) { return each * c + more * c / parts; };   // total c / parts
+  CaPlace p{{a.n_seq, 0, 0, 0}, {0, 0, 0, 0, 0, 0}, 0, 0};
+  const int u = cut(cta + (ends ? 1 : 0));
   if (cta < parts) {
-    long long before = 0;
+    int before = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
       if (a.n_seq > 32) before = group.load(a, s0 + lane, rep, lane, before);
-      ca_locate(a, group, s0, u0, rep, lane, begin, unused);
-      ca_locate(a, group, s0, u1, rep, lane, end, rest);
+      ca_locate(a, group, s0, u, rep, lane, p);
     }
   }
-  if (lane == 0) {
-    sh->begin = begin;
-    sh->end = end;
-    if (a.head != nullptr) {
-      int4 head = make_int4(0, 0, 0, 0);
-      if (end.tile > 0 && (!begin.same_block(end) || begin.tile == 0)) {
-        CaSeq q;
-        q.load(a, end.seq, rep);
-        // the block's last unit is u1 + rest - 1, in the last CTA j with total j / parts < u1 + rest
-        head.x = (int)(((u1 + rest) * parts - 1) / total - cta) + 1;
-        head.y = q.base;
-        head.z = end.blk * kCaBlock;
-        head.w = q.block_rows(end.blk) | end.kvh << 16;
+  if (!ends) {
+    if (lane == 0) {
+      sh->begin = p.at;
+      sh->begin_seq = p.q;
+    }
+    return;
+  }
+  if (lane == 0) sh->end = p.at;
+  if (a.head == nullptr) return;
+  int4 head = make_int4(0, 0, 0, 0);
+  // the block that is cut at u begins in this CTA: at its first tile, of which a unit may lie in front
+  if (p.at.tile > 0 && cut(cta) < u - p.within + (p.q.dual(p.at.blk) ? 1 : 2)) {
+    for (int j0 = cta + 1; j0 < parts; j0 += 32) {
+      const unsigned int closed = __ballot_sync(0xffffffffu, j0 + lane < parts && cut(j0 + lane + 1) >= u + p.left);
+      if (closed != 0) {
+        head.x = j0 + __ffs(closed) - cta;
+        break;
       }
-      a.head[cta] = head;
     }
+    head.y = p.q.base;
+    head.z = p.at.blk * kCaBlock;
+    head.w = p.q.block_rows(p.at.blk) | p.at.kvh << 16;
   }
+  if (lane == 0) a.head[cta] = head;
 }
 
 // The blocks of a CTA's part one after the other; every warp walks for itself.
@@ -232,7 +230,7 @@ struct CaWalk {
   }
   __device__ __forceinline__ bool first(const ChunkArgs& a, const CaShared* sh, int rep) {
     at = sh->begin;
-    if (at.seq < a.n_seq) q.load(a, at.seq, rep);
+    q = sh->begin_seq;
     return enter(a, sh, rep);
   }
   __device__ __forceinline__ bool next(const ChunkArgs& a, const CaShared* sh, int rep) {
@@ -357,7 +355,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rep = a.Hq / a.Hkv;
   pdl_launch();
   const WaitReport report{&sh->dead, &g_chunk_failures, a.failed};
-  if (warp == 0) ca_span(a, sh, rep, lane);
+  if (warp < 2) ca_span(a, sh, rep, lane, warp == 1);
   if (warp == 12) {
     if (elect_one()) {
       mbar_init(&sh->q_full, 2);
@@ -523,7 +521,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         const long long part = 2ll * blockIdx.x + (w.t0 > 0 ? 0 : 1);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f, f0 = own_f * inv, f1 = other_f * inv;
         bf16* const orow = a.out + (long long)(w.q.base + token) * a.ldo + (long long)(w.at.kvh * rep + h) * D;
-        float* const prow = a.part + (part * a.part_rows + row) * D;
+        float4* const prow = a.part + part * (D / 4) * a.part_rows + row;
         if (!whole && is_row) a.ml[part * a.part_rows + row] = make_float2(m2, l);
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
@@ -545,9 +543,8 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
 #pragma unroll
               for (int i = 0; i < 32; i += 8) dst[i / 8] = make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]), pack_bf16(o[i + 6], o[i + 7]));
             } else {
-              float4* dst = reinterpret_cast<float4*>(prow + c0);
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 4) prow[(long long)((c0 + i) / 4) * a.part_rows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
           }
           __syncwarp();                                  // the next load of tensor memory wants the whole warp
@@ -638,10 +635,14 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       uint32_t seg = 0;
       for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep), ++seg) {
         if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report)) break;
+        int token = (w.row0 + r0) / rep, h = w.row0 + r0 - token * rep;
+        const bf16* src = a.q + (long long)(w.q.base + token) * a.ldq + (long long)(w.at.kvh * rep + h) * D + c * 8;
+        const long long wrap = a.ldq - (long long)rep * D;
+#pragma unroll 4
         for (int r = r0; r < w.n_rows; r += kAt) {
-          const int token = (w.row0 + r) / rep, h = w.row0 + r - token * rep;
-          const bf16* src = a.q + (long long)(w.q.base + token) * a.ldq + (long long)(w.at.kvh * rep + h) * D + c * 8;
           cp_async16(qs + (r >> 7) * C::kQTile + (c >> 3) * kCaQBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, true);
+          src += kAt * D;
+          for (h += kAt; h >= rep; h -= rep) src += wrap;
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -660,75 +661,58 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   }
 }
 
-// The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A warp takes some rows, one after
-// the other; nothing but the number of parts is waited for before the loads.
+// The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A thread has eight dimensions of a
+// row, neighbouring threads neighbouring rows.
 template <int D>
-__global__ void __launch_bounds__(32 * kCaJoinWarps) chunk_attn_join_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(kCaJoinThreads) chunk_attn_join_kernel(const ChunkArgs a) {
   pdl_wait();
-  constexpr int E = D / 32;
-  const int i = blockIdx.x, lane = threadIdx.x & 31, rep = a.Hq / a.Hkv;
+  const int i = blockIdx.x, rep = a.Hq / a.Hkv;
   const int4 head = a.head[i];
-  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16;
-  if (parts == 0) return;
-  for (int r = 0; r < kCaJoinRows; ++r) {
-    const int row = (blockIdx.y * kCaJoinRows + r) * kCaJoinWarps + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    auto at = [&](int k) { return (2ll * (i + k) + (k == 0 ? 1 : 0)) * a.part_rows + row; };
-    float top = -INFINITY, l = 0.f, acc[E];
+  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16, id = blockIdx.y * kCaJoinThreads + threadIdx.x;
+  const int group = id / max(rows, 1), row = id - group * rows;
+  if (parts == 0 || group >= D / 8) return;
+  float top = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      float2 mine = make_float2(-INFINITY, 0.f);
-      if (k0 + lane < parts) mine = a.ml[at(k0 + lane)];
-      const int here = min(32, parts - k0);
-      float4 ahead[4];                                   // the first parts' numbers, before their factors are known
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  constexpr int kAhead = 8;                              // parts whose loads are under way together
+  for (int k0 = 0; k0 < parts; k0 += kAhead) {
+    float2 m[kAhead];
+    float4 u[kAhead], v[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float* o = a.part + at(k0 + min(k, here - 1)) * D + lane * E;
-        if constexpr (E == 4) ahead[k] = *reinterpret_cast<const float4*>(o);
-        else ahead[k] = make_float4(o[0], o[1], 0.f, 0.f);
-      }
-      float most = mine.x;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = ca_max3(most, __shfl_xor_sync(0xffffffffu, most, o), most);
-      most = ca_max3(most, top, most);
-      const float before = top == -INFINITY ? 0.f : ca_ex2(top - most), f = mine.x == -INFINITY ? 0.f : ca_ex2(mine.x - most);
-      top = most;
-      l = l * before + f * mine.y;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = before == 0.f ? 0.f : acc[e] * before;
-      auto add = [&](int k, const float4& v) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        if (fk == 0.f) return;                           // a part in which the row saw no key
-        acc[0] += v.x * fk;
-        acc[1] += v.y * fk;
-        if constexpr (E == 4) {
-          acc[2] += v.z * fk;
-          acc[3] += v.w * fk;
-        }
-      };
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < here) add(k, ahead[k]);
-#pragma unroll 4
-      for (int k = 4; k < here; ++k) {
-        const float* o = a.part + at(k0 + k) * D + lane * E;
-        add(k, E == 4 ? *reinterpret_cast<const float4*>(o) : make_float4(o[0], o[1], 0.f, 0.f));
-      }
+    for (int k = 0; k < kAhead; ++k) {
+      const long long part = 2ll * (i + min(k0 + k, parts - 1)) + (k0 + k == 0 ? 1 : 0);
+      m[k] = a.ml[part * a.part_rows + row];
+      u[k] = a.part[(part * (D / 4) + 2 * group) * a.part_rows + row];
+      v[k] = a.part[(part * (D / 4) + 2 * group + 1) * a.part_rows + row];
+      if (k0 + k >= parts) m[k].x = -INFINITY;
     }
-    l = warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int token = (head.z + row) / rep, h = head.z + row - token * rep;
-    bf16* out = a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + lane * E;
-    if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-    else *reinterpret_cast<uint32_t*>(out) = pack_bf16(acc[0] * inv, acc[1] * inv);
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) most = ca_max3(most, m[k].x, most);
+    const float before = top == -INFINITY ? 0.f : ca_ex2(top - most);
+    top = most;
+    l *= before;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= before;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (m[k].x == -INFINITY) continue;                 // no part, or one in which the row saw no key
+      const float f = ca_ex2(m[k].x - most);
+      l += f * m[k].y;
+      acc[0] += f * u[k].x, acc[1] += f * u[k].y, acc[2] += f * u[k].z, acc[3] += f * u[k].w;
+      acc[4] += f * v[k].x, acc[5] += f * v[k].y, acc[6] += f * v[k].z, acc[7] += f * v[k].w;
+    }
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int token = (head.z + row) / rep, h = head.z + row - token * rep;
+  *reinterpret_cast<uint4*>(a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + group * 8) =
+      make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv), pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
 }
 
 // ---------------------------------------------------------------------------------------------------- host
 struct CaPlan {
   int grid, part_rows;
-  bool cut;                // whether a block can be cut
+  bool cut, fits;          // whether a block can be cut; whether the products can be counted in 31 bits
   long long bytes;
 };
 static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
@@ -736,6 +720,7 @@ static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int 
   const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * (tiles > 1 ? tiles : 1);   // products there can be
   const long long parts = most / kCaMinUnits;
   CaPlan p;
+  p.fits = most < (1ll << 31);
   const int sms = num_sms();
   p.grid = parts < 1 ? 1 : (parts < sms ? (int)parts : sms);
   p.part_rows = rows < kCaBlock ? (int)rows : kCaBlock;
@@ -761,8 +746,8 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   int rc = check_launch("omc_paged_chunk_attn");
   if (rc != OMC_OK || !plan.cut) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(plan.grid, (plan.part_rows + kCaJoinRows * kCaJoinWarps - 1) / (kCaJoinRows * kCaJoinWarps));
-  cfg.blockDim = dim3(32 * kCaJoinWarps);
+  cfg.gridDim = dim3(plan.grid, (plan.part_rows * (D / 8) + kCaJoinThreads - 1) / kCaJoinThreads);
+  cfg.blockDim = dim3(kCaJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -808,6 +793,7 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
     return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: null pointer");
   const long long reach = (long long)max_pages * page_size;
   const CaPlan plan = ca_plan(n_seq, max_new, max_ctx, Hq, Hkv, head_dim);
+  if (!plan.fits) return set_error(OMC_ERR_SHAPE, "omc_paged_chunk_attn: 2^31 products of 128 rows and 64 keys or more: fewer sequences, rows or positions per call");
   if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
     return set_error(OMC_ERR_ARG, "omc_paged_chunk_attn: workspace missing, too small or not on a 16-byte boundary");
   ChunkArgs a{};
@@ -817,7 +803,7 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
   if (plan.bytes > 0) {
     a.head = static_cast<int4*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.head + plan.grid);
-    a.part = reinterpret_cast<float*>(a.ml + 2ll * plan.grid * plan.part_rows);
+    a.part = reinterpret_cast<float4*>(a.ml + 2ll * plan.grid * plan.part_rows);
     a.part_rows = plan.part_rows;
   }
   rc = step_failure_word(&a.failed);
