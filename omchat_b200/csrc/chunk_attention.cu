@@ -391,9 +391,9 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
     constexpr int kLanes = D / 8, kPer = 32 / kLanes, kOwn = kCaKeys / 4;   // lanes of a row, rows of a warp at a time, rows of a warp
     const int c = lane % kLanes, sub = lane / kLanes;
     int slot = 0;
-    uint32_t parity = 1;
+    uint32_t parity = 1, seg = 0;
     bool go = true;
-    for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep)) {
+    for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep), ++seg) {
       const int32_t* bt = a.table + (long long)w.at.seq * a.max_pages;
       for (int tile = w.t0; go && tile < w.t1; ++tile) {
         const int key = tile * kCaKeys + warp * kOwn + lane;
@@ -402,7 +402,9 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
           const int index = key / a.page_size, page = bt[index];
           if (page >= 0 && page < a.n_pages) row = (page * 2 * a.Hkv + w.at.kvh) * a.page_size + key - index * a.page_size;
         }
-        go = wait_bounded_warp(&sh->empty[slot], parity, report);
+        // an SM takes in some 46 bytes a cycle: 256 rows of queries come before more tiles than the first two
+        if (!w.dual && tile == w.t0 + 2) go = wait_bounded_warp(&sh->q_full, seg & 1u, report);
+        go = go && wait_bounded_warp(&sh->empty[slot], parity, report);
         if (!go) break;
 #pragma unroll 1
         for (int values = 0; values < 2; ++values) {
@@ -630,19 +632,22 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       }
     } else {
       // ---------------------------------------------------------------------------------------- queries
-      constexpr int kLanes = D / 8, kAt = 64 / kLanes;
-      const int c = (tid - 448) % kLanes, r0 = (tid - 448) / kLanes;
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+      const int c = lane % kLanes, sub = lane / kLanes, tile = warp - 14;
+      uint8_t* const dst = qs + tile * C::kQTile + (c >> 3) * kCaQBox;
       uint32_t seg = 0;
       for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep), ++seg) {
         if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report)) break;
-        int token = (w.row0 + r0) / rep, h = w.row0 + r0 - token * rep;
-        const bf16* src = a.q + (long long)(w.q.base + token) * a.ldq + (long long)(w.at.kvh * rep + h) * D + c * 8;
-        const long long wrap = a.ldq - (long long)rep * D;
+        const bf16* const head = a.q + (long long)w.at.kvh * rep * D + c * 8;
+        for (int r0 = 0; tile * kCaRows + r0 < w.n_rows && r0 < kCaRows; r0 += 32) {
+          // a lane finds a row's place, all of them fetch it
+          const int mine = w.row0 + min(tile * kCaRows + r0 + lane, w.n_rows - 1), token = mine / rep;
+          const long long place = (long long)(w.q.base + token) * a.ldq + (mine - token * rep) * D;
 #pragma unroll 4
-        for (int r = r0; r < w.n_rows; r += kAt) {
-          cp_async16(qs + (r >> 7) * C::kQTile + (c >> 3) * kCaQBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, true);
-          src += kAt * D;
-          for (h += kAt; h >= rep; h -= rep) src += wrap;
+          for (int i = 0; i < 32 / kPer; ++i) {
+            const int r = r0 + i * kPer + sub;
+            cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), head + __shfl_sync(0xffffffffu, place, r - r0), true);
+          }
         }
         cp_async_commit();
         cp_async_wait<0>();
