@@ -549,9 +549,27 @@ def paged_decode_attn(qkv, inv_freq, kv_pool, block_table, page_size, ctx_lens, 
 
 
 # ---- going on with cached sequences by a chunk of new tokens (csrc/rotary.cu, csrc/chunk_attention.cu)
-def _ask(ok: bool, what: str):
-    if not ok:
-        raise OmcError(what)
+_I32, _F64, _BF16 = torch.int32, torch.float64, torch.bfloat16
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int, dtype, what: str) -> int:
+    """The row stride of t, which is [rows, cols] of dtype with the elements of a row side by side."""
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.stride(1) != 1:
+        raise OmcError(f"{what} is {dtype} [{rows}, {cols}] with the elements of a row side by side, not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+    return t.stride(0)
+
+
+def _vector(t: torch.Tensor, n: int, dtype, what: str):
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+        raise OmcError(f"{what} is contiguous {dtype} [{n}], not {t.dtype} {tuple(t.shape)}")
+
+
+def _paged(kv_pool: torch.Tensor, block_table: torch.Tensor):
+    if kv_pool.dtype is not _BF16 or kv_pool.dim() != 5 or kv_pool.shape[1] != 2 or not kv_pool.is_contiguous():
+        raise OmcError("the pool is contiguous bfloat16 [pages, 2, kv heads, page, head]")
+    if block_table.dtype is not _I32 or block_table.dim() != 2 or not block_table.is_contiguous():
+        raise OmcError("the block table is contiguous int32 [sequences, pages]")
+    return kv_pool.shape
 
 
 def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, head_dim: int, *, halves: bool = True, back: bool = False,
@@ -559,44 +577,41 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, 
     """Rotary positions of rows x [T, heads * head_dim] (bf16 or fp32, row-strided) at positions pos (int32 [T]); out may be x. turns: float64
     [rotated dims / 2], see rope.frequencies(); halves: pairs (i, i + rotated / 2) instead of (2i, 2i + 1); back: by the negative angle."""
     _need_cuda(x, pos, turns, out)
-    T = x.shape[0]
-    _ask(x.dim() == 2 and x.shape[1] == heads * head_dim and x.stride(1) == 1 and x.dtype in (torch.bfloat16, torch.float32),
-         "rotary: x is [rows, heads * head_dim] of bfloat16 or float32, elements of a row side by side")
-    _ask(pos.dtype == torch.int32 and pos.shape == (T,) and pos.is_contiguous(), "rotary: pos is int32 [rows]")
-    _ask(turns.dtype == torch.float64 and turns.dim() == 1 and turns.is_contiguous(), "rotary: turns is float64 [rotated dims / 2]")
+    dtype, T = x.dtype, x.shape[0]
+    if dtype is not _BF16 and dtype is not torch.float32:
+        raise OmcError(f"rotary: rows of bfloat16 or float32, not {dtype}")
+    ldx = _rows(x, T, heads * head_dim, dtype, "rotary: x")
+    _vector(pos, T, _I32, "rotary: pos")
+    n = turns.numel()
+    _vector(turns, n, _F64, "rotary: turns")
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    _ask(out.shape == x.shape and out.dtype == x.dtype and out.stride(1) == 1, "rotary: out is like x")
-    rc = load().omc_rotary_rows(x, 1 if x.dtype == torch.float32 else 0, x.stride(0), pos, T, heads, head_dim, turns, 2 * turns.shape[0], 1 if halves else 0,
-                                1 if back else 0, mscale, out, out.stride(0), _stream())
+        out = torch.empty_like(x)
+    ldy = _rows(out, T, heads * head_dim, dtype, "rotary: out")
+    rc = load().omc_rotary_rows(x, 0 if dtype is _BF16 else 1, ldx, pos, T, heads, head_dim, turns, 2 * n, 1 if halves else 0, 1 if back else 0, mscale, out, ldy,
+                                _stream())
     _check(rc, "omc_rotary_rows")
     return out
-
-
-def _check_paged(kv_pool: torch.Tensor, block_table: torch.Tensor, what: str):
-    _ask(kv_pool.dim() == 5 and kv_pool.shape[1] == 2 and kv_pool.dtype == torch.bfloat16 and kv_pool.is_contiguous(),
-         f"{what}: the pool is bfloat16 [pages, 2, kv heads, page, head]")
-    _ask(block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.is_contiguous(), f"{what}: the table is int32 [sequences, pages]")
 
 
 def rotary_kv_append(qkv: torch.Tensor, pos: torch.Tensor, seq_ids: Optional[torch.Tensor], turns: torch.Tensor, Hq: int, kv_pool: torch.Tensor,
                      block_table: torch.Tensor, *, halves: bool = True, mscale: float = 1.0, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """qkv [T, (Hq + 2 Hkv) * head] bf16: rotated queries -> the result (q_out, or new rows; qkv's own columns are fine), rotated keys and values -> the
-    cache rows (seq_ids[t], pos[t]) of kv_pool [pages, 2, Hkv, page, head]. Rows without a place in the table (sequence -1: padding) are not appended."""
+    cache rows (seq_ids[t], pos[t]) of kv_pool [pages, 2, Hkv, page, head]. Rows without a place in the table (sequence -1: padding) are not appended; no two
+    rows may have the same place."""
     _need_cuda(qkv, pos, seq_ids, turns, kv_pool, block_table, q_out)
-    _check_paged(kv_pool, block_table, "rotary_kv_append")
-    n_pages, _, Hkv, page, head = kv_pool.shape
+    n_pages, _, Hkv, page, head = _paged(kv_pool, block_table)
     T = qkv.shape[0]
-    _ask(qkv.dim() == 2 and qkv.shape[1] == (Hq + 2 * Hkv) * head and qkv.stride(1) == 1 and qkv.dtype == torch.bfloat16,
-         "rotary_kv_append: qkv is bfloat16 [rows, (q heads + 2 kv heads) * head], elements of a row side by side")
-    _ask(pos.dtype == torch.int32 and pos.shape == (T,) and pos.is_contiguous(), "rotary_kv_append: pos is int32 [rows]")
-    _ask(seq_ids is None or (seq_ids.dtype == torch.int32 and seq_ids.shape == (T,) and seq_ids.is_contiguous()), "rotary_kv_append: seq_ids is int32 [rows]")
-    _ask(turns.dtype == torch.float64 and turns.dim() == 1 and turns.is_contiguous(), "rotary_kv_append: turns is float64 [rotated dims / 2]")
+    ld = _rows(qkv, T, (Hq + 2 * Hkv) * head, _BF16, "rotary_kv_append: qkv")
+    _vector(pos, T, _I32, "rotary_kv_append: pos")
+    if seq_ids is not None:
+        _vector(seq_ids, T, _I32, "rotary_kv_append: seq_ids")
+    n = turns.numel()
+    _vector(turns, n, _F64, "rotary_kv_append: turns")
     if q_out is None:
-        q_out = torch.empty(T, Hq * head, device=qkv.device, dtype=torch.bfloat16)
-    _ask(q_out.shape == (T, Hq * head) and q_out.dtype == torch.bfloat16 and q_out.stride(1) == 1, "rotary_kv_append: q_out is bfloat16 [rows, q heads * head]")
-    rc = load().omc_rotary_kv_append(qkv, qkv.stride(0), pos, seq_ids, T, Hq, Hkv, head, turns, 2 * turns.shape[0], 1 if halves else 0, mscale, q_out,
-                                     q_out.stride(0), kv_pool, n_pages, block_table, block_table.shape[0], block_table.shape[1], page, _stream())
+        q_out = qkv.new_empty((T, Hq * head))
+    rc = load().omc_rotary_kv_append(qkv, ld, pos, seq_ids, T, Hq, Hkv, head, turns, 2 * n, 1 if halves else 0, mscale, q_out,
+                                     _rows(q_out, T, Hq * head, _BF16, "rotary_kv_append: q_out"), kv_pool, n_pages, block_table, block_table.shape[0],
+                                     block_table.shape[1], page, _stream())
     _check(rc, "omc_rotary_kv_append")
     return q_out
 
@@ -607,20 +622,22 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
     the last positions of the ctx_lens[s] that sequence s has. max_new / max_ctx: what no sequence has more of (host numbers; the lengths
     themselves stay on the device). Rows behind cu_new[-1] are not written."""
     _need_cuda(q, kv_pool, block_table, cu_new, ctx_lens, out)
-    _check_paged(kv_pool, block_table, "paged_attention")
-    n_pages, _, Hkv, page, head = kv_pool.shape
-    n_seq = block_table.shape[0]
-    _ask(q.dim() == 2 and q.shape[1] == Hq * head and q.stride(1) == 1 and q.dtype == torch.bfloat16, "paged_attention: q is bfloat16 [rows, q heads * head]")
-    _ask(cu_new.dtype == torch.int32 and cu_new.shape == (n_seq + 1,) and cu_new.is_contiguous() and ctx_lens.dtype == torch.int32
-         and ctx_lens.shape == (n_seq,) and ctx_lens.is_contiguous(), "paged_attention: cu_new is int32 [sequences + 1], ctx_lens int32 [sequences]")
+    n_pages, _, Hkv, page, head = _paged(kv_pool, block_table)
+    n_seq, max_pages = block_table.shape
+    T = q.shape[0]
+    ldq = _rows(q, T, Hq * head, _BF16, "paged_attention: q")
+    _vector(cu_new, n_seq + 1, _I32, "paged_attention: cu_new")
+    _vector(ctx_lens, n_seq, _I32, "paged_attention: ctx_lens")
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
-    _ask(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(1) == 1, "paged_attention: out is like q")
-    need = load().omc_paged_chunk_attn_workspace_bytes(n_seq, max_new, max_ctx, Hq, Hkv, head)
-    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
-    rc = load().omc_paged_chunk_attn(q, q.stride(0), kv_pool, n_pages, block_table, block_table.shape[1], page, cu_new, ctx_lens, n_seq, q.shape[0], max_new,
-                                     max_ctx, Hq, Hkv, head, scale, out, out.stride(0), ws, need, _stream())
+        out = torch.empty_like(q)
+    L = load()
+    need = L.omc_paged_chunk_attn_workspace_bytes(n_seq, max_new, max_ctx, Hq, Hkv, head)
+    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None   # of this call alone: calls of other streams and graphs have their own
+    rc = L.omc_paged_chunk_attn(q, ldq, kv_pool, n_pages, block_table, max_pages, page, cu_new, ctx_lens, n_seq, T, max_new, max_ctx, Hq, Hkv, head, scale, out,
+                                _rows(out, T, Hq * head, _BF16, "paged_attention: out"), ws, need, _stream())
     _check(rc, "omc_paged_chunk_attn")
+    if ws is not None:
+        add_launches(1)
     return out
 
 
