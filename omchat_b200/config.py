@@ -64,6 +64,7 @@ class OmChatQwen2Config:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 1e6
     max_position_embeddings: int = 32768
+    rope_scaling: Optional[dict] = None      # as in config.json (rope.frequencies): linear, yarn or llama3
     # multimodal attributes read by the reference
     mm_vision_tower: Optional[str] = "InternViT-6B-448px-V1-5"
     mm_projector_type: str = "mlp2x_gelu"

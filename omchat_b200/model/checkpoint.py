@@ -22,9 +22,10 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from ..config import FofisunConfig, InternVisionConfig, MunevikConfig, OmChatQwen2Config, OmChatQwen2MoeConfig, SorupelConfig, TifisunConfig, VefunexConfig, VoduzenConfig
+from ..rope import kind
 
 _TEXT_KEYS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_layers", "num_attention_heads",
-              "num_key_value_heads", "rms_norm_eps", "rope_theta", "max_position_embeddings")
+              "num_key_value_heads", "rms_norm_eps", "rope_theta", "max_position_embeddings", "rope_scaling")
 _MM_KEYS = ("mm_vision_tower", "mm_projector_type", "mm_hidden_size", "mm_vision_select_layer",
             "mm_vision_select_feature", "image_grid_pinpoints", "tokenizer_model_max_length", "tokenizer_padding_side",
             "tune_mm_mlp_adapter", "mm_use_im_start_end", "eos_token_id", "pad_token_id", "mm_pixel_shuffle_ratio",
@@ -54,6 +55,12 @@ def config_from_dict(d: dict) -> OmChatQwen2Config:
     for k in _TEXT_KEYS:
         if text.get(k) is not None:
             kw[k] = text[k]
+    rope = text.get("rope_parameters")
+    if isinstance(rope, dict):  # newer config.json: the base and the scaling in one dictionary
+        if rope.get("rope_theta") is not None:
+            kw["rope_theta"] = rope["rope_theta"]
+        if kind(rope) != "default":
+            kw.setdefault("rope_scaling", {k: v for k, v in rope.items() if k != "rope_theta"})
     for k in _MM_KEYS:
         if d.get(k) is not None:
             kw[k] = d[k]

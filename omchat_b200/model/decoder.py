@@ -36,7 +36,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from .. import lib
+from .. import lib, rope
 from ..config import OmChatQwen2Config
 from .weights import LlmW
 
@@ -54,8 +54,11 @@ MEGA_HIST = 4096  # token-history rows kept on the device between host reads
 
 
 def rope_inv_freq(cfg: OmChatQwen2Config, device) -> torch.Tensor:
-    """Qwen2RotaryEmbedding default init (modeling_qwen2.py:51-100): computed on the host in fp32 exactly as HF does."""
+    """Qwen2RotaryEmbedding default init (modeling_qwen2.py:51-100): computed on the host in fp32 exactly as HF does; stretched
+    frequencies (rope_scaling) from rope.frequencies()."""
     d = cfg.head_dim
+    if rope.kind(cfg.rope_scaling) != "default":
+        return (rope.frequencies(d, cfg.rope_theta, cfg.rope_scaling)[0] * (2 * math.pi)).to(torch.float32).to(device)
     inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, d, 2, dtype=torch.int64).to(torch.float32) / d))
     return inv.to(device)
 
@@ -124,7 +127,10 @@ class Qwen2Decoder:
         dense = [l for l in w.layers if l.gate_up_w is not None]
         self.I_local = dense[0].gate_up_w.shape[0] // 2 if dense else 8  # 8: placeholder width when every layer is sparse
         self.V_local = w.lm_head.shape[0]
-        self.scale = cfg.head_dim ** -0.5
+        # Frequencies in turns for the rows of a chunk (lib.rotary_kv_append). A factor on cosine and sine (yarn) multiplies queries and keys alike: it is left out of
+        # both, squared into the scale of the scores, so that every kernel that writes or reads the cache agrees.
+        self.turns, mscale = rope.frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, self.device)
+        self.scale = cfg.head_dim ** -0.5 * mscale * mscale
         self.eps = cfg.rms_norm_eps
         self.mega_enabled = os.environ.get("OMCHAT_B200_NO_MEGA", "0") != "1"
         # batched decode steps (B > 4): weight-streaming GEMMs on packed weights (0 = the skinny GEMM / GEMV path)
@@ -266,15 +272,41 @@ class Qwen2Decoder:
         assert max(lens) <= cache.capacity, "KV cache too small for this prefill"
         dev = embeds.device
         cu = torch.tensor(list(offsets), dtype=torch.int32).to(dev, non_blocking=True)
+        Hq, Hkv, max_len = self.Hq, self.Hkv, max(lens)
+
+        def attend(li, qkv, attn):
+            lib.rope_kv_store(qkv, pos_ids, seq_ids, Hq, Hkv, self.inv_freq, cache.pool[li], cache.block_table,
+                              cache.page_size)
+            lib.attention(qkv[:, :Hq * 128], qkv[:, Hq * 128:(Hq + Hkv) * 128], qkv[:, (Hq + Hkv) * 128:], attn, cu,
+                          max_len, Hq, Hkv, True, self.scale)
+
         h = embeds[:T].clone() if self.tp.size > 1 else embeds[:T]  # residual stream, updated in place
-        C, Hq, Hkv = self.C, self.Hq, self.Hkv
-        qw = (Hq + 2 * Hkv) * 128
+        hiddens = self._layer_rows(h, attend, collect_hidden)
+        if slots is None:
+            cache.host_lens = list(lens)
+            cache.ctx_lens.copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
+        else:
+            for s_, n_ in zip(slots, lens):
+                cache.host_lens[s_] = n_
+            cache.ctx_lens.copy_(torch.tensor(cache.host_lens, dtype=torch.int32), non_blocking=True)
+        out = self._row_logits(h, offsets, logits)
+        return (out, hiddens) if collect_hidden else out
+
+    def _row_logits(self, h, offsets, logits: str):
+        if logits == "last":
+            last_rows = torch.tensor([offsets[i + 1] - 1 for i in range(len(offsets) - 1)], dtype=torch.int64).to(h.device)
+            return self.lm_head(h.index_select(0, last_rows))
+        return self.lm_head(h) if logits == "all" else None
+
+    def _layer_rows(self, h, attend, collect_hidden: bool = False):
+        """All layers over the packed rows h [T, C] (in place); attend(layer, qkv, attn) rotates q|k|v, appends k and v to the cache and leaves the
+        attention's rows in attn. Returns the hidden states if asked."""
+        T, C, dev = h.shape[0], self.C, h.device
         xn = torch.empty(T, C, device=dev, dtype=torch.bfloat16)
-        qkv = torch.empty(T, qw, device=dev, dtype=torch.bfloat16)
-        attn = torch.empty(T, Hq * 128, device=dev, dtype=torch.bfloat16)
+        qkv = torch.empty(T, (self.Hq + 2 * self.Hkv) * 128, device=dev, dtype=torch.bfloat16)
+        attn = torch.empty(T, self.Hq * 128, device=dev, dtype=torch.bfloat16)
         act = torch.empty(T, self.I_local, device=dev, dtype=torch.bfloat16)
         hiddens = [h.clone()] if collect_hidden else None
-        max_len = max(lens)
         fold = self.fold_norms
         if fold:
             # input / post-attention RMSNorm folded into the qkv / gate|up GEMMs (omc_gemm_bf16_norm): o_proj / down_proj leave
@@ -288,10 +320,7 @@ class Qwen2Decoder:
             else:
                 lib.rmsnorm(h, l.ln1, self.eps, out=xn)
                 lib.gemm(xn, l.qkv_w, out=qkv, bias=l.qkv_b)
-            lib.rope_kv_store(qkv, pos_ids, seq_ids, Hq, Hkv, self.inv_freq, cache.pool[li], cache.block_table,
-                              cache.page_size)
-            lib.attention(qkv[:, :Hq * 128], qkv[:, Hq * 128:(Hq + Hkv) * 128], qkv[:, (Hq + Hkv) * 128:], attn, cu,
-                          max_len, Hq, Hkv, True, self.scale)
+            attend(li, qkv, attn)
             self._row_parallel(attn, l.o_w, h, use_gemv=False, ssq_out=ssq_b if fold else None)
             if fold:
                 lib.gemm(h, folded[li][1], out=act, epi=lib.EPI_SWIGLU, ssq_in=ssq_b, norm_dim=C, eps=self.eps)
@@ -300,20 +329,71 @@ class Qwen2Decoder:
                 self._mlp_rows(li, l, h, xn, act)
             if collect_hidden:
                 hiddens.append(h.clone())
-        if slots is None:
-            cache.host_lens = list(lens)
-            cache.ctx_lens.copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
+        return hiddens
+
+    # ------------------------------------------------------------------------------------------------ going on with cached sequences
+    def _few_rows(self, T: int) -> bool:
+        """Whether a chunk of T rows goes through the weight-streaming GEMMs of the batched decode step (overridden where a layer has other parts)."""
+        return self.stream_enabled and self.tp.size == 1 and T <= 64
+
+    def _layer_rows_stream(self, h, attend):
+        """_layer_rows for at most 64 rows: the launches of a batched decode step around attend()."""
+        P, C, T, dev = self.packed_weights(), self.C, h.shape[0], h.device
+        parts = lib.ssq_parts(C)
+        qkv = torch.empty(T, (self.Hq + 2 * self.Hkv) * 128, device=dev, dtype=torch.bfloat16)
+        attn = torch.empty(T, self.Hq * 128, device=dev, dtype=torch.bfloat16)
+        act = torch.empty(T, self.I_local, device=dev, dtype=torch.bfloat16)
+        ssq_a, ssq_b = torch.zeros(2, parts * 64, device=dev, dtype=torch.float32)
+        lib.row_ssq(h, ssq_a, parts=parts, pdl=False)
+        for li, (l, p) in enumerate(zip(self.w.layers, P.layers)):
+            lib.gemm_stream(h, p.qkv, out=qkv, bias=l.qkv_b, ssq_in=ssq_a, ssq_in_parts=parts, norm_dim=C, eps=self.eps)
+            attend(li, qkv, attn)
+            lib.gemm_stream(attn, p.o, out=h, res=h, epi=lib.EPI_RES, ssq_out=ssq_b)
+            lib.gemm_stream(h, p.gate_up, out=act, epi=lib.EPI_SWIGLU, ssq_in=ssq_b, ssq_in_parts=parts, norm_dim=C, eps=self.eps)
+            lib.gemm_stream(act, p.down, out=h, res=h, epi=lib.EPI_RES, ssq_out=ssq_a)
+
+    @torch.no_grad()
+    def extend(self, embeds: torch.Tensor, offsets: Sequence[int], cache: PagedKVCache, logits: str = "last", collect_hidden: bool = False,
+               slots: Optional[Sequence[int]] = None):
+        """Goes on with cached sequences by a chunk of new tokens each (none, one or many): rows offsets[i] .. offsets[i + 1] of embeds [T, C] bf16 follow
+        the cache.host_lens positions that cache row i (slots[i]) has. An empty row is a fresh prompt, so a prompt can be given in portions of any size.
+        `logits` as in prefill(); 'last' of a sequence without new tokens is not defined and refused."""
+        n_seq, T = len(offsets) - 1, offsets[-1]
+        rows = list(range(n_seq)) if slots is None else [int(s) for s in slots]
+        lens = [offsets[i + 1] - offsets[i] for i in range(n_seq)]
+        if offsets[0] != 0 or min(lens, default=0) < 0 or embeds.shape[0] < T:
+            raise ValueError("offsets begin at 0, do not fall, and end within the rows of embeds")
+        if len(rows) != n_seq or (slots is None and n_seq != cache.n_seq) or len(set(rows)) != n_seq or any(not 0 <= s < cache.n_seq for s in rows):
+            raise ValueError("one different row of the cache for every sequence of the chunk")
+        ends = [cache.host_lens[s] + n for s, n in zip(rows, lens)]
+        if max(ends, default=0) > cache.capacity:
+            raise ValueError(f"KV cache is full: {max(ends)} positions of {cache.capacity}")
+        if logits == "last" and min(lens, default=0) == 0:
+            raise ValueError("a sequence without new tokens has no last row: ask for logits='all' or 'none'")
+        if T == 0:
+            return (None, None) if collect_hidden else None
+        dev, Hq = embeds.device, self.Hq
+        # positions | cache rows | first rows | contexts | cache rows of the sequences, in one copy
+        pos = [torch.arange(e - n, e, dtype=torch.int32) for e, n in zip(ends, lens)]
+        seq = [torch.full((n,), s, dtype=torch.int32) for s, n in zip(rows, lens)]
+        meta = torch.cat([*pos, *seq, torch.tensor([*offsets, *ends, *rows], dtype=torch.int32)]).to(dev)
+        pos_ids, seq_ids, cu, ctx, which = meta.split([T, T, n_seq + 1, n_seq, n_seq])
+        table = cache.block_table if rows == list(range(cache.n_seq)) else cache.block_table.index_select(0, which)
+        max_new, max_ctx = max(lens), max(ends)
+
+        def attend(li, qkv, attn):
+            q = lib.rotary_kv_append(qkv, pos_ids, seq_ids, self.turns, Hq, cache.pool[li], cache.block_table, q_out=qkv[:, :Hq * 128])
+            lib.paged_attention(q, cache.pool[li], table, cu, ctx, max_new, max_ctx, Hq, self.scale, out=attn)
+
+        h, hiddens = embeds[:T].clone(), None
+        if self._few_rows(T) and not collect_hidden:
+            self._layer_rows_stream(h, attend)
         else:
-            for s_, n_ in zip(slots, lens):
-                cache.host_lens[s_] = n_
-            cache.ctx_lens.copy_(torch.tensor(cache.host_lens, dtype=torch.int32), non_blocking=True)
-        out = None
-        if logits == "last":
-            last_rows = torch.tensor([offsets[i + 1] - 1 for i in range(n_seq)], dtype=torch.int64).to(dev)
-            hl = h.index_select(0, last_rows)
-            out = self.lm_head(hl)
-        elif logits == "all":
-            out = self.lm_head(h)
+            hiddens = self._layer_rows(h, attend, collect_hidden)
+        for s, e in zip(rows, ends):
+            cache.host_lens[s] = e
+        cache.ctx_lens.copy_(torch.tensor(cache.host_lens, dtype=torch.int32), non_blocking=True)
+        out = self._row_logits(h, offsets, logits)
         return (out, hiddens) if collect_hidden else out
 
     # the MLP half of a layer on the per-op paths (overridden by the mixture-of-experts decoder, model/moe.py)

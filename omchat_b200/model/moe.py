@@ -41,6 +41,9 @@ class Qwen2MoeDecoder(Qwen2Decoder):
         self._moe_ws = {}
         self._rcat = {}
 
+    def _few_rows(self, T: int) -> bool:
+        return False  # the streaming step of a sparse layer belongs to _decode_body_stream
+
     def _workspace(self, T: int) -> lib.MoeWorkspace:
         """One workspace per power-of-two token bucket, shared by all layers (allocated outside graph capture: the first,
         uncaptured step of generate_greedy creates it)."""

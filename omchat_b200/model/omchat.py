@@ -305,15 +305,20 @@ class OmChatQwen2ForCausalLM:
                 logits_to_keep: Union[int, str] = 0):
         """omchat_qwen2.py:45-89. Prefill: input_ids [b,S] (with -200 placeholders) + images [n,3,448,448] -> logits
         [b,T,V] fp32 padded like the reference pads (positions outside the mask are zero). Decode step: input_ids
-        [b,1] + past_key_values -> logits [b,1,V]. `max_cache_len` sizes the paged cache of a prefill (default: T +
+        [b,1] + past_key_values -> logits [b,1,V]. Several new tokens: input_ids [b,n] (with images, if they hold placeholders) or
+        inputs_embeds [b,n,C] + past_key_values -> logits [b,T,V] of the new positions, behind those that the cache has; an
+        attention_mask of the new tokens, or one whose last n columns are theirs, says which of them are there. `max_cache_len` sizes the paged cache of a prefill (default: T +
         generation_config.max_new_tokens); `logits_to_keep=1` computes only each sequence's last position."""
         if output_attentions:
             raise NotImplementedError("attention probabilities are never materialised by the flash kernels")
         dec = self.model.decoder
         # ---- decode step (omchat_arch.py:59-70 short-circuit)
         if past_key_values is not None and past_key_values.get_seq_length() > 0:
-            if inputs_embeds is not None or input_ids is None or input_ids.shape[1] != 1:
-                raise ValueError("with a populated cache, forward() takes exactly one new token per sequence")
+            if inputs_embeds is not None or images is not None or (input_ids is not None and input_ids.shape[1] != 1):
+                return self._forward_chunk(input_ids, attention_mask, past_key_values, inputs_embeds, labels, output_hidden_states, images, return_dict,
+                                           logits_to_keep)
+            if input_ids is None:
+                raise ValueError("You have to specify either input_ids or inputs_embeds")
             logits = self._gather_vocab(dec.decode_step(input_ids.to(self.device).reshape(-1), past_key_values).clone())
             return self._output(logits[:, None, :], past_key_values, None, return_dict)
         # ---- prefill
@@ -371,6 +376,38 @@ class OmChatQwen2ForCausalLM:
         if hiddens is not None:
             hs = tuple(self._pad(x, offsets) for x in hiddens)
         return self._output(logits, past_key_values if use_cache is not False else None, loss, return_dict, hs)
+
+    def _forward_chunk(self, input_ids, attention_mask, cache, inputs_embeds, labels, output_hidden_states, images, return_dict, logits_to_keep):
+        """forward() with several new tokens per sequence behind a populated cache (modeling_qwen2.py:341-411 with past_key_values)."""
+        if labels is not None:
+            raise ValueError("labels go with a whole prompt, not with a populated cache")
+        if input_ids is None and inputs_embeds is None:
+            raise ValueError("You have to specify either input_ids or inputs_embeds")
+        new = input_ids if inputs_embeds is None else inputs_embeds
+        b, n = new.shape[:2]
+        if b != cache.n_seq:
+            raise ValueError(f"{b} sequences, and a cache of {cache.n_seq}")
+        mask = attention_mask
+        if mask is not None:
+            if mask.shape[0] != b or mask.shape[1] < n:
+                raise ValueError(f"an attention_mask of {tuple(mask.shape)} for {b} x {n} new tokens")
+            mask = mask[:, mask.shape[1] - n:]
+        if inputs_embeds is None:
+            embeds, _, _, offsets = self._splice_packed(input_ids.to(self.device), mask, images)
+        else:
+            inputs_embeds = inputs_embeds.to(device=self.device, dtype=torch.bfloat16)
+            lens = [n] * b if mask is None else mask.bool().sum(1).tolist()
+            embeds = inputs_embeds.reshape(b * n, -1) if mask is None else inputs_embeds[mask.to(self.device).bool()]
+            offsets = [0]
+            for m in lens:
+                offsets.append(offsets[-1] + m)
+        mode = "last" if logits_to_keep == 1 else "all"
+        res = self.model.decoder.extend(embeds, offsets, cache, logits=mode, collect_hidden=bool(output_hidden_states))
+        logits, hiddens = res if output_hidden_states else (res, None)
+        logits = self._gather_vocab(logits)
+        logits = logits[:, None, :] if mode == "last" else self._pad(logits, offsets)
+        hs = None if hiddens is None else tuple(self._pad(x, offsets) for x in hiddens)
+        return self._output(logits, cache, None, return_dict, hs)
 
     __call__ = forward
 

@@ -43,18 +43,24 @@ class _Request:
     out: List[int] = field(default_factory=list)
     pages: List[int] = field(default_factory=list)
     done: bool = False
+    embeds: Optional[torch.Tensor] = None   # rows of a prompt that goes in by portions, until the last one is in
+    filled: int = 0                          # of them in the cache
 
 
 class ContinuousBatcher:
     """model: OmChatQwen2ForCausalLM (single GPU). slots: decode batch (1..64). max_ctx: longest prompt + generation a slot
     can hold. total_pages: size of the shared page pool (default: enough for every slot at max_ctx). chunk: decode steps
-    between two looks at the host side (admission, EOS, release)."""
+    between two looks at the host side (admission, EOS, release). prefill_chunk: prompts of more rows go in by portions of so
+    many, one between two chunks of decode steps, so that a long prompt holds up the other slots by a portion at a time."""
 
-    def __init__(self, model, slots: int = 4, max_ctx: int = 4096, total_pages: Optional[int] = None, chunk: int = 8):
+    def __init__(self, model, slots: int = 4, max_ctx: int = 4096, total_pages: Optional[int] = None, chunk: int = 8,
+                 prefill_chunk: Optional[int] = None):
         if not 1 <= slots <= MAX_SLOTS:
             raise ValueError(f"slots must be 1..{MAX_SLOTS}")
+        if prefill_chunk is not None and prefill_chunk < 1:
+            raise ValueError("prefill_chunk must be >= 1")
         self.model, self.dec = model, model.model.decoder
-        self.slots, self.chunk = slots, chunk
+        self.slots, self.chunk, self.prefill_chunk = slots, chunk, prefill_chunk
         ps = model.config.kv_page_size
         # one page more per slot than max_ctx needs: the pool then holds every slot at full length PLUS the scratch page
         self.cache: PagedKVCache = self.dec.new_cache(slots, max_ctx + ps, shuffle_pages=False)
@@ -107,9 +113,10 @@ class ContinuousBatcher:
     def step(self):
         """Admit what fits, then one chunk of decode steps for all slots, then retire what finished."""
         self._admit()
-        live = [r for r in self.active if r is not None]
+        self._fill()
+        live = [r for r in self.active if r is not None and r.embeds is None]
         if not live:
-            if self.queue:
+            if self.queue and all(r is None for r in self.active):
                 raise RuntimeError("a queued request does not fit the page pool even when it is empty")
             return
         n = min(self.chunk, min(r.max_new - len(r.out) for r in live))
@@ -118,7 +125,7 @@ class ContinuousBatcher:
             self.steps_run += n
             self.cur = toks[:, -1].to(self.model.device)
             for s, r in enumerate(self.active):
-                if r is None:
+                if r is None or r.embeds is not None:
                     continue
                 for t in toks[s].tolist():
                     r.out.append(t)
@@ -145,16 +152,44 @@ class ContinuousBatcher:
             self.table_host[s].fill_(self.scratch)
             self.table_host[s, :need] = torch.tensor(r.pages, dtype=torch.int32)
             self.cache.block_table.copy_(self.table_host)
-            seq.fill_(s)  # the packed rows of this request belong to cache row s
-            logits = self.dec.prefill(embeds, pos, seq, offsets, self.cache, logits="last", slots=[s])
-            first = lib.argmax(logits)
-            t0 = int(first[0])
-            r.out.append(t0)
-            if (r.eos is not None and t0 == r.eos) or r.max_new == 1:
-                r.done = True
-            self.cur[s] = first[0]
+            if self.prefill_chunk is not None and T > self.prefill_chunk:
+                r.embeds = embeds[:T]
+            else:
+                seq.fill_(s)  # the packed rows of this request belong to cache row s
+                self._first_token(s, r, self.dec.prefill(embeds, pos, seq, offsets, self.cache, logits="last", slots=[s]))
             self.active[s] = r
         self._retire()
+
+    def _first_token(self, s: int, r: _Request, logits: torch.Tensor):
+        first = lib.argmax(logits)
+        t0 = int(first[0])
+        r.out.append(t0)
+        if (r.eos is not None and t0 == r.eos) or r.max_new == 1:
+            r.done = True
+        self.cur[s] = first[0]
+
+    def _fill(self):
+        """One portion for every slot whose prompt is not in the cache yet. Between portions such a slot is an idle one for the decode
+        steps: scratch page, context 0."""
+        filling = [(s, r) for s, r in enumerate(self.active) if r is not None and r.embeds is not None]
+        for s, r in filling:
+            n = min(self.prefill_chunk, r.embeds.shape[0] - r.filled)
+            self.table_host[s, :len(r.pages)] = torch.tensor(r.pages, dtype=torch.int32)
+            self.cache.block_table.copy_(self.table_host)
+            self.cache.host_lens[s] = r.filled
+            last = r.filled + n == r.embeds.shape[0]
+            logits = self.dec.extend(r.embeds[r.filled:r.filled + n], [0, n], self.cache, logits="last" if last else "none", slots=[s])
+            r.filled += n
+            if last:
+                r.embeds = None
+                self._first_token(s, r, logits)
+            else:
+                self.table_host[s].fill_(self.scratch)
+                self.cache.host_lens[s] = 0
+        if filling:
+            self.cache.block_table.copy_(self.table_host)
+            self.cache.ctx_lens.copy_(torch.tensor(self.cache.host_lens, dtype=torch.int32))
+            self._retire()
 
     def _retire(self):
         changed = False
@@ -169,13 +204,13 @@ class ContinuousBatcher:
         # idle slots: scratch page, context 0 (the kernel still runs them: it appends to the scratch page and its
         # samples are ignored); live slots keep their lengths
         for s, r in enumerate(self.active):
-            if r is None and self.cache.host_lens[s] != 0:
+            if (r is None or r.embeds is not None) and self.cache.host_lens[s] != 0:
                 self.cache.host_lens[s] = 0
                 changed = True
         if changed:
             self.cache.block_table.copy_(self.table_host)
             self.cache.ctx_lens.copy_(torch.tensor(self.cache.host_lens, dtype=torch.int32))
-            self.cur = torch.where(torch.tensor([r is not None for r in self.active], device=self.cur.device), self.cur,
+            self.cur = torch.where(torch.tensor([r is not None and r.embeds is None for r in self.active], device=self.cur.device), self.cur,
                                    torch.zeros_like(self.cur))
 
 
