@@ -31,8 +31,11 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int kCaRows = 128, kCaKeys = 64, kCaBlock = 256, kCaThreads = 512;
 constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
-constexpr int kCaMinUnits = 2;           // products (128 rows x 64 keys) a CTA has at least: one of each stream, some 2 us. A single token behind 1087 positions: 8 units
-                                         // 16.4 us, 2 units JOIN_US
+// Products (128 rows x 64 keys) a CTA has at least where blocks are cut: one of each stream. A single token behind 1087 positions, replayed: 16.4 us with 8, 13.1 with 2,
+// 12.1 with 1, which a token behind 2000 loses again (14.4 against 12.3).
+constexpr int kCaMinUnits = 2;
+// Products of a block up to which none is cut and there is no second kernel: 10.5 us against 12.5 for a token behind 300 positions, 18 against 12.7 behind 900.
+constexpr int kCaWhole = 6;
 constexpr int kCaJoinThreads = 256;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
@@ -74,7 +77,7 @@ struct CaSeq {
     return max(0, min(ctx, ctx - n_all + token + 1));
   }
   __device__ __forceinline__ int tiles(int b, int rep) const { return max(1, (keys(b, rep) + kCaKeys - 1) / kCaKeys); }
-  __device__ __forceinline__ int units(int b, int rep) const { return tiles(b, rep) * (dual(b) ? 1 : 2); }
+  __device__ __forceinline__ int units(int b, int rep, bool cut) const { return cut ? tiles(b, rep) * (dual(b) ? 1 : 2) : 1; }
 };
 
 struct CaPos {
@@ -124,12 +127,12 @@ struct CaGroup {
   __device__ __forceinline__ int load(const ChunkArgs& a, int s, int rep, int lane, int before) {   // the units up to the group's end
     q = CaSeq{0, 0, 0, 0, 0, 0};
     if (s < a.n_seq) q.load(a, s, rep);
-    one = q.blocks == 1 ? q.units(0, rep) : 0;
+    one = q.blocks == 1 ? q.units(0, rep, a.head != nullptr) : 0;
     for (unsigned int many = __ballot_sync(0xffffffffu, q.blocks > 1); many != 0; many &= many - 1) {
       const int from = __ffs(many) - 1;
       const CaSeq w = ca_shfl(q, from);
       int sum = 0;
-      for (int b = lane; b < w.blocks; b += 32) sum += w.units(b, rep);
+      for (int b = lane; b < w.blocks; b += 32) sum += w.units(b, rep, a.head != nullptr);
       sum = ca_warp_sum(sum);
       if (lane == from) one = sum;
     }
@@ -154,7 +157,7 @@ __device__ __forceinline__ void ca_locate(const ChunkArgs& a, const CaGroup& gro
   p.within = u - start - p.at.kvh * per;
   p.at.blk = 0;
   for (int b0 = 0; b0 < p.q.blocks; b0 += 32) {
-    const int b = b0 + lane, mine = b < p.q.blocks ? p.q.units(b, rep) : 0, up = ca_warp_scan(mine, lane);
+    const int b = b0 + lane, mine = b < p.q.blocks ? p.q.units(b, rep, a.head != nullptr) : 0, up = ca_warp_scan(mine, lane);
     const unsigned int in = __ballot_sync(0xffffffffu, p.within < up);
     if (in != 0) {
       const int l = __ffs(in) - 1, all = __shfl_sync(0xffffffffu, up, l), own = __shfl_sync(0xffffffffu, mine, l);
@@ -172,7 +175,7 @@ __device__ __forceinline__ void ca_span(const ChunkArgs& a, CaShared* sh, int re
   CaGroup group;
   int total = 0;
   for (int s0 = 0; s0 < a.n_seq; s0 += 32) total = group.load(a, s0 + lane, rep, lane, total);
-  const int parts = min((int)gridDim.x, max(1, total / kCaMinUnits)), cta = blockIdx.x, each = total / parts, more = total - each * parts;
+  const int parts = min((int)gridDim.x, max(1, a.head != nullptr ? total / kCaMinUnits : total)), cta = blockIdx.x, each = total / parts, more = total - each * parts;
   auto cut = [&](int c) { return each * c + more * c / parts; };   // total c / parts
   CaPlace p{{a.n_seq, 0, 0, 0}, {0, 0, 0, 0, 0, 0}, 0, 0};
   const int u = cut(cta + (ends ? 1 : 0));
@@ -395,13 +398,23 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
     bool go = true;
     for (bool more = w.first(a, sh, rep); go && more; more = w.next(a, sh, rep), ++seg) {
       const int32_t* bt = a.table + (long long)w.at.seq * a.max_pages;
-      for (int tile = w.t0; go && tile < w.t1; ++tile) {
+      // Of a tile: the page of the lane's row, or -1, and the row in it. Looked up a tile ahead.
+      auto look_up = [&](int tile, int& page, int& in_page) {
         const int key = tile * kCaKeys + warp * kOwn + lane;
-        int row = -1;                                    // of the pool, in rows of D
-        if (lane < kOwn && key < w.keys) {
-          const int index = key / a.page_size, page = bt[index];
-          if (page >= 0 && page < a.n_pages) row = (page * 2 * a.Hkv + w.at.kvh) * a.page_size + key - index * a.page_size;
+        page = -1;
+        if (tile < w.t1 && lane < kOwn && key < w.keys) {
+          const int index = key / a.page_size;
+          in_page = key - index * a.page_size;
+          page = bt[index];
         }
+      };
+      int page, in_page = 0, next_page, next_in_page = 0;
+      look_up(w.t0, page, in_page);
+      for (int tile = w.t0; go && tile < w.t1; ++tile) {
+        look_up(tile + 1, next_page, next_in_page);
+        const int row = page >= 0 && page < a.n_pages ? (page * 2 * a.Hkv + w.at.kvh) * a.page_size + in_page : -1;   // of the pool, in rows of D
+        page = next_page;
+        in_page = next_in_page;
         // an SM takes in some 46 bytes a cycle: 256 rows of queries come before more tiles than the first two
         if (!w.dual && tile == w.t0 + 2) go = wait_bounded_warp(&sh->q_full, seg & 1u, report);
         go = go && wait_bounded_warp(&sh->empty[slot], parity, report);
@@ -667,9 +680,9 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
 }
 
 // The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A thread has eight dimensions of a
-// row, neighbouring threads neighbouring rows.
-template <int D>
-__global__ void __launch_bounds__(kCaJoinThreads) chunk_attn_join_kernel(const ChunkArgs a) {
+// row, neighbouring threads neighbouring rows, AHEAD parts' loads under way together.
+template <int D, int AHEAD>
+__global__ void __launch_bounds__(kCaJoinThreads, AHEAD > 4 ? 1 : 4) chunk_attn_join_kernel(const ChunkArgs a) {
   pdl_wait();
   const int i = blockIdx.x, rep = a.Hq / a.Hkv;
   const int4 head = a.head[i];
@@ -679,12 +692,11 @@ __global__ void __launch_bounds__(kCaJoinThreads) chunk_attn_join_kernel(const C
   float top = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  constexpr int kAhead = 8;                              // parts whose loads are under way together
-  for (int k0 = 0; k0 < parts; k0 += kAhead) {
-    float2 m[kAhead];
-    float4 u[kAhead], v[kAhead];
+  for (int k0 = 0; k0 < parts; k0 += AHEAD) {
+    float2 m[AHEAD];
+    float4 u[AHEAD], v[AHEAD];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
+    for (int k = 0; k < AHEAD; ++k) {
       const long long part = 2ll * (i + min(k0 + k, parts - 1)) + (k0 + k == 0 ? 1 : 0);
       m[k] = a.ml[part * a.part_rows + row];
       u[k] = a.part[(part * (D / 4) + 2 * group) * a.part_rows + row];
@@ -693,14 +705,14 @@ __global__ void __launch_bounds__(kCaJoinThreads) chunk_attn_join_kernel(const C
     }
     float most = top;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) most = ca_max3(most, m[k].x, most);
+    for (int k = 0; k < AHEAD; ++k) most = ca_max3(most, m[k].x, most);
     const float before = top == -INFINITY ? 0.f : ca_ex2(top - most);
     top = most;
     l *= before;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] *= before;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
+    for (int k = 0; k < AHEAD; ++k) {
       if (m[k].x == -INFINITY) continue;                 // no part, or one in which the row saw no key
       const float f = ca_ex2(m[k].x - most);
       l += f * m[k].y;
@@ -721,15 +733,16 @@ struct CaPlan {
   long long bytes;
 };
 static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
-  const long long rows = (long long)max_new * (Hq / Hkv), tiles = ((long long)max_ctx + kCaKeys - 1) / kCaKeys;
-  const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * (tiles > 1 ? tiles : 1);   // products there can be
-  const long long parts = most / kCaMinUnits;
+  const long long rows = (long long)max_new * (Hq / Hkv), tiles = max_ctx <= kCaKeys ? 1 : ((long long)max_ctx + kCaKeys - 1) / kCaKeys;
+  const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * tiles, blocks = (long long)n_seq * Hkv * ((rows + kCaBlock - 1) / kCaBlock);
   CaPlan p;
   p.fits = most < (1ll << 31);
+  p.cut = tiles * (rows > kCaRows ? 2 : 1) > kCaWhole;
+  const long long parts = p.cut ? most / kCaMinUnits : blocks;
   const int sms = num_sms();
   p.grid = parts < 1 ? 1 : (parts < sms ? (int)parts : sms);
+  p.cut = p.cut && p.grid > 1;
   p.part_rows = rows < kCaBlock ? (int)rows : kCaBlock;
-  p.cut = p.grid > 1 && tiles > 1;
   p.bytes = p.cut ? (long long)p.grid * 16 + 2ll * p.grid * p.part_rows * (8 + 4ll * head_dim) : 0;
   return p;
 }
@@ -759,7 +772,8 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D>, a);
+  // few rows are cut into many parts; many rows into two or three, and need the registers for threads (512 rows behind 4096: 54 us against 57 with eight)
+  const cudaError_t e = plan.part_rows <= 64 ? cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 8>, a) : cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 3>, a);
   if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");
 }
