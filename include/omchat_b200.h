@@ -220,7 +220,9 @@ int omc_rotary_kv_append(const void* qkv, long long ldqkv, const int32_t* pos, c
  * max_new and max_ctx: what no sequence has more of (rows beyond max_new are not computed, positions beyond max_ctx or the table not read); the device reads
  * the lengths itself, so a captured call goes by the lengths of its replay. Pages outside the pool read as zeros. Keys and values behind ctx_lens[s] may
  * hold anything; a value that is not finite reaches the rows of its sequence that are computed beside those that see it (as many as share a tile).
- * workspace: omc_paged_chunk_attn_workspace_bytes(...) bytes (0: NULL is fine), 16-byte aligned, nothing in it outlives the call. */
+ * workspace: omc_paged_chunk_attn_workspace_bytes(...) bytes (0: NULL is fine), 16-byte aligned, nothing in it outlives the call. Its kernel's waits end by
+ * themselves; after one that ran out what was computed is not valid: omc_wait_failed() says 1 (without waiting for the device), and launches are refused. */
+int omc_wait_failed(void);
 long long omc_paged_chunk_attn_workspace_bytes(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim);
 int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv_pool, int n_pages, const int32_t* block_table, int max_pages, int page_size,
                          const int32_t* cu_new, const int32_t* ctx_lens, int n_seq, int T, int max_new, int max_ctx, int Hq, int Hkv, int head_dim,

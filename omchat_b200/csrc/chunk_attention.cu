@@ -52,6 +52,7 @@ struct ChunkArgs {
   long long ldo;
   int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, Hq, Hkv;
   float scale_log2;
+  int wide;                // out is on 32-byte boundaries, its rows too
   int4* head;              // workspace: [CTAs] (parts of the block that is cut behind this CTA or 0, first row of q, first row of the block, rows | key/value head << 16)
   float2* ml;              // [2 CTAs][part_rows] maximum (base 2, scaled) and sum
   float4* part;            // [2 CTAs][D / 4][part_rows]: the threads of a warp have neighbouring rows
@@ -282,6 +283,10 @@ __device__ __forceinline__ float ca_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// A whole sector: neighbouring threads have rows far apart, and 16 bytes at a time cost an SM as much of its way to L2.
+__device__ __forceinline__ void ca_store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 // The maximum keeps a NaN: it then is the row's reference, and the row becomes NaN whichever unit its exponentials come from.
 __device__ __forceinline__ float ca_max3(float a, float b, float c) {
@@ -554,9 +559,17 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
           }
           if (is_row) {
             if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+              uint32_t w16[16];
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) dst[i / 8] = make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]), pack_bf16(o[i + 6], o[i + 7]));
+              for (int i = 0; i < 16; ++i) w16[i] = pack_bf16(o[2 * i], o[2 * i + 1]);
+              if (a.wide) {
+                ca_store32(orow + c0, w16);
+                ca_store32(orow + c0 + 16, w16 + 8);
+              } else {
+                uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w16[4 * i], w16[4 * i + 1], w16[4 * i + 2], w16[4 * i + 3]);
+              }
             } else {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) prow[(long long)((c0 + i) / 4) * a.part_rows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -650,7 +663,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       uint8_t* const dst = qs + tile * C::kQTile + (c >> 3) * kCaQBox;
       uint32_t seg = 0;
       for (bool more = w.first(a, sh, rep); more; more = w.next(a, sh, rep), ++seg) {
-        if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report)) break;
+        if (seg > 0 && !wait_bounded_warp(&sh->q_empty, (seg - 1u) & 1u, report, kWaitTries << 5)) break;   // for all tiles of a block, the other waits are for one
         const bf16* const head = a.q + (long long)w.at.kvh * rep * D + c * 8;
         for (int r0 = 0; tile * kCaRows + r0 < w.n_rows && r0 < kCaRows; r0 += 32) {
           // a lane finds a row's place, all of them fetch it
@@ -791,6 +804,13 @@ static int ca_check(int n_seq, int T, int max_new, int max_ctx, int Hq, int Hkv,
   return OMC_OK;
 }
 
+extern "C" int omc_wait_failed(void) {
+  const volatile unsigned int* words = step_failure_words();
+  int any = 0;
+  for (int dev = 0; words != nullptr && dev < kMaxDevices; ++dev) any |= words[dev] != 0u;
+  return any;
+}
+
 extern "C" long long omc_paged_chunk_attn_workspace_bytes(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
   const int rc = ca_check(n_seq, 0, max_new, max_ctx, Hq, Hkv, head_dim);
   return rc != OMC_OK ? rc : ca_plan(n_seq, max_new, max_ctx, Hq, Hkv, head_dim).bytes;
@@ -819,6 +839,7 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
   a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.pool = static_cast<const bf16*>(kv_pool); a.table = block_table; a.cu = cu_new; a.ctx = ctx_lens;
   a.out = static_cast<bf16*>(out); a.ldo = ldo; a.n_seq = n_seq; a.T = T; a.max_new = max_new; a.max_ctx = reach < max_ctx ? (int)reach : max_ctx;
   a.n_pages = n_pages; a.max_pages = max_pages; a.page_size = page_size; a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * 1.4426950408889634f;
+  a.wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && ldo % 16 == 0;
   if (plan.bytes > 0) {
     a.head = static_cast<int4*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.head + plan.grid);

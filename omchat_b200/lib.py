@@ -67,6 +67,7 @@ SIGNATURES = {
     "omc_paged_decode_attn": (_I, [_P, _L, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _F, _P, _L, _P, _P]),
     "omc_rotary_rows": (_I, [_P, _I, _L, _P, _I, _I, _I, _P, _I, _I, _I, _F, _P, _L, _P]),
     "omc_rotary_kv_append": (_I, [_P, _L, _P, _P, _I, _I, _I, _I, _P, _I, _I, _F, _P, _L, _P, _I, _P, _I, _I, _I, _P]),
+    "omc_wait_failed": (_I, []),
     "omc_paged_chunk_attn_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I]),
     "omc_paged_chunk_attn": (_I, [_P, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _L, _P]),
     "omc_embed_lookup": (_I, [_P, _I, _P, _I, _P, _L, _I, _P]),
@@ -639,6 +640,13 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
     if ws is not None:
         add_launches(1)
     return out
+
+
+def check_waits():
+    """Raises if a wait of paged_attention's kernel has run out: what was computed since is not valid. Does not synchronise - call it behind whatever
+    waited for the results."""
+    if _lib is not None and _lib.omc_wait_failed():
+        raise OmcError("a wait of the paged attention's kernel ran out; what was computed since is not valid")
 
 
 def embed_lookup(ids: torch.Tensor, table: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

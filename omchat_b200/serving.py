@@ -163,6 +163,7 @@ class ContinuousBatcher:
     def _first_token(self, s: int, r: _Request, logits: torch.Tensor):
         first = lib.argmax(logits)
         t0 = int(first[0])
+        lib.check_waits()
         r.out.append(t0)
         if (r.eos is not None and t0 == r.eos) or r.max_new == 1:
             r.done = True
