@@ -279,6 +279,8 @@ template <int R>
 __device__ __forceinline__ void ca_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int N>
 __device__ __forceinline__ void ca_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ void ca_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 __device__ __forceinline__ float ca_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
     // ------------------------------------------------------------------------------------------ softmax and epilogue
     ca_regs_up<kCaRegsSoftmax>();
     const int t = (warp - 4) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;   // TMEM lanes go by warp % 4
-    const int both = 1 + quarter;                        // barrier of the two warps of the same lanes
+    const int both = 1 + quarter, turn = 5 + quarter;    // barriers of the two warps of the same lanes
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, to = tmem + lanes + 256u;
     const float sl2 = a.scale_log2, grown = 8.f / sl2;
     // the lanes of a warp may leave a wait one by one, and accesses to tensor memory are the warp's as a whole; whether the phase came is not asked
@@ -463,6 +465,10 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
       const bool any = row - lane < w.n_rows, is_row = row < w.n_rows;
       const int token = (w.row0 + row) / rep, h = w.row0 + row - token * rep, p = w.q.ctx - w.q.n_all + token;
       float m = -INFINITY, l = 0.f;
+      // The two warps of the same lanes of TMEM are of one scheduler: they take turns in the exponentials, so that one's scores, maxima and waits lie under the other's.
+      // Left alone they fall into step, and both take longer.
+      const bool turns = !w.dual && kCaRows + quarter * 32 < w.n_rows;
+      if (turns && t == 1) ca_arrive<64>(turn);
       for (int i = 0; i < mine; ++i, ++done) {
         const uint32_t ts = tmem + lanes + (uint32_t)(t * 128) + (done & 1u) * kCaKeys;
         wait(&sh->s_full[t][done & 1u], done >> 1 & 1u);
@@ -496,7 +502,9 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
           }
           const float neg = m == -INFINITY ? 0.f : -m * sl2;
           const uint64_t sl2_2 = ca_f2(sl2, sl2), neg_2 = ca_f2(neg, neg);
+          if (turns) ca_sync<64>(turn + 4 * t);
           l += ca_probabilities(v, ts, sl2_2, neg_2);
+          if (turns && (t == 0 || i + 1 < mine)) ca_arrive<64>(turn + 4 - 4 * t);
           if (rescale && i > 0) {
             product(done - 1u);
             tc_fence_after();
