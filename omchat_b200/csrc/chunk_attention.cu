@@ -290,7 +290,7 @@ __device__ __forceinline__ float ca_ex2(float x) {
 __device__ __forceinline__ void ca_store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// The maximum keeps a NaN: it then is the row's reference, and the row becomes NaN whichever unit its exponentials come from.
+// The maximum keeps a NaN, which then is the row's reference.
 __device__ __forceinline__ float ca_max3(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -312,25 +312,9 @@ __device__ __forceinline__ uint64_t ca_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x of two numbers on the multiply-add pipe: n = round(x) by adding 1.5 2^23, 2^(x - n) on [-1/2, 1/2] by the polynomial of degree 3 whose largest relative
-// error is least (Remez; 7.5e-5, a fiftieth of what P is rounded to), n added to the exponent. Below 2^-126 it stays there.
-__device__ __forceinline__ void ca_ex2_fma(float x0, float x1, float& e0, float& e1) {
-  const uint64_t x = ca_f2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t t = ca_add2(x, ca_f2(12582912.f, 12582912.f));
-  const uint64_t f = ca_fma2(ca_add2(t, ca_f2(-12582912.f, -12582912.f)), ca_f2(-1.f, -1.f), x);
-  uint64_t p = ca_fma2(ca_f2(0.0551716685f, 0.0551716685f), f, ca_f2(0.242611125f, 0.242611125f));
-  p = ca_fma2(p, f, ca_f2(0.693260968f, 0.693260968f));
-  p = ca_fma2(p, f, ca_f2(0.999928057f, 0.999928057f));
-  float t0, t1, p0, p1;
-  ca_f2(t, t0, t1);
-  ca_f2(p, p0, p1);
-  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
-// 2^(v sl2 + neg) of a row's scores, rounded to bf16 into tensor memory from column ts on; their sum, before the rounding. Two of eight pairs leave the
-// exponential unit (8 cycles of a scheduler per instruction) to the others. Measured at 2048 rows behind 28672: none 845 us, one 828, two 815, three 827. A hidden
-// score is 2^-126 there and not zero, which changes no sum that has a visible one in it.
+// 2^(v sl2 + neg) of a row's scores, rounded to bf16 into tensor memory from column ts on; their sum, before the rounding. All on the exponential unit (8 cycles of a
+// scheduler per instruction): a polynomial on the multiply-add pipe for a quarter of them was a gain while both streams computed theirs at the same time (815 us
+// against 845 for 2048 rows behind 28672), and is a loss where they take turns (750 against 723): its instructions are three times as many.
 __device__ __forceinline__ float ca_probabilities(const uint32_t (&v)[kCaKeys], uint32_t ts, uint64_t sl2, uint64_t neg) {
   uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
@@ -341,9 +325,7 @@ __device__ __forceinline__ float ca_probabilities(const uint32_t (&v)[kCaKeys], 
       const int at = b * 32 + 2 * i;
       float x0, x1;
       ca_f2(ca_fma2(ca_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl2, neg), x0, x1);
-      float e0, e1;
-      if ((i & 3) == 0) ca_ex2_fma(x0, x1, e0, e1);
-      else e0 = ca_ex2(x0), e1 = ca_ex2(x1);
+      const float e0 = ca_ex2(x0), e1 = ca_ex2(x1);
       sum[i & 3] = ca_add2(sum[i & 3], ca_f2(e0, e1));
       pk[i] = pack_bf16(e0, e1);
     }
@@ -525,7 +507,6 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
         if (lane == 0) mbar_arrive(&sh->p_ready[t][done & 1u]);
       }
       if (mine > 0) product(done - 1u);                  // and all in front of it, of the same accumulator
-      if (m == -INFINITY) l = 0.f;                       // no visible key
       tc_fence_after();
       float own_f = 1.f, other_f = 0.f, m2 = m * sl2;    // m2: in base 2
       bool two = false;
