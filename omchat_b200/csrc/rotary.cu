@@ -86,8 +86,8 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a) {
 
 // The same by pieces of 16 bytes, a block per row: a thread has one piece of a head (of a rotated part in halves one of either half) and waits for it while the block works
 // out the row's sines, rot / 2 of them for all heads. Bound by HBM, with waits in a row's life that only other rows on the SM can fill: 32 registers, so that 2048
-// threads are there. 32768 rows of 32 heads of 128: 92 us = 5.8 TB/s, 0.90 of a copy's rate; with two rows per block 97 us, with four (and fewer blocks) 119. 16384 rows
-// of 28 + 2 x 4 heads appended: 64 us = 4.8 TB/s.
+// threads are there. 32768 rows of 32 heads of 128: 105 us = 5.1 TB/s, 0.79 of a copy's rate (two rows per block 109, four 119; blocks that stay and fetch the next
+// row ahead 100 to 108). 16384 rows of 28 + 2 x 4 heads appended: 65 us = 4.6 TB/s (66 to 78).
 template <typename TT, bool HALVES>
 __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs a, int lanes_log2) {
   constexpr int V = 16 / (int)sizeof(TT);                // elements of a piece

@@ -554,10 +554,10 @@ _I32, _F64, _BF16 = torch.int32, torch.float64, torch.bfloat16
 
 
 def _rows(t: torch.Tensor, rows: int, cols: int, dtype, what: str) -> int:
-    """The row stride of t, which is [rows, cols] of dtype with the elements of a row side by side."""
+    """The row stride of t, which is [rows, cols] of dtype with the elements of a row side by side (of one row: any number would do)."""
     if t.dtype is not dtype or t.shape != (rows, cols) or t.stride(1) != 1:
         raise OmcError(f"{what} is {dtype} [{rows}, {cols}] with the elements of a row side by side, not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
-    return t.stride(0)
+    return t.stride(0) if rows > 1 else cols
 
 
 def _vector(t: torch.Tensor, n: int, dtype, what: str):
@@ -621,7 +621,7 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
                     max_ctx: int, Hq: int, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of the new tokens of every sequence over the cache that holds them already: rows cu_new[s] .. cu_new[s + 1] of q [T, Hq * head] are
     the last positions of the ctx_lens[s] that sequence s has. max_new / max_ctx: what no sequence has more of (host numbers; the lengths
-    themselves stay on the device). Rows behind cu_new[-1] are not written."""
+    themselves stay on the device). Rows behind cu_new[-1] are not written. out may be q."""
     _need_cuda(q, kv_pool, block_table, cu_new, ctx_lens, out)
     n_pages, _, Hkv, page, head = _paged(kv_pool, block_table)
     n_seq, max_pages = block_table.shape

@@ -150,6 +150,51 @@ def test_replay_goes_by_the_lengths_of_the_replay():
         assert bool((out[sum(n):] == 5).all())
 
 
+def test_pools_beyond_31_bits():
+    """Pages whose rows lie behind 2^31 elements and 2^32 bytes of the pool, written and read."""
+    hq, hkv, head, page, c = 14, 2, 128, 64, 9000
+    n_pages = (1 << 31) // (2 * hkv * page * head) + 200
+    pool = torch.empty(n_pages, 2, hkv, page, head, dtype=BF, device="cuda")
+    per, g = -(-c // page), torch.Generator().manual_seed(2)
+    table = (n_pages - 1 - torch.randperm(per, generator=g)).to(torch.int32).view(1, per).cuda()
+    qkv = torch.randn(c, (hq + 2 * hkv) * head, generator=g).to(BF).cuda()
+    pos, turns = torch.arange(c, dtype=torch.int32).cuda(), torch.rand(64, dtype=torch.float64, generator=g).cuda()
+    q = lib.rotary_kv_append(qkv, pos, None, turns, hq, pool, table)
+    for n in (1, 300):
+        cu, lens = torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([c], dtype=torch.int32).cuda()
+        out = lib.paged_attention(q[c - n:], pool, table, cu, lens, n, c, hq, 0.088)
+        _check(out, q[c - n:], pool, table, [n], [c], hq, hkv, head, 0.088)
+    at = table[0, (pos // page).long()].long()
+    assert torch.equal(pool[at, 1, :, (pos % page).long()], qkv.view(c, -1, head)[:, hq + hkv:])
+
+
+def test_many_sequences():
+    """More sequences than a warp has lanes, most of them short or empty, and one long one in a later group."""
+    new = [(i * 7) % 4 for i in range(150)]
+    ctx = [n + (i * 13) % 200 for i, n in enumerate(new)]
+    new[97], ctx[97] = 60, 3000
+    q, pool, table, cu, lens = _inputs(new, ctx, 14, 2, 64, 16)
+    out = lib.paged_attention(q, pool, table, cu, lens, 60, 3000, 14, 0.125)
+    _check(out, q, pool, table, new, ctx, 14, 2, 64, 0.125)
+
+
+def test_queries_and_results_in_the_same_rows():
+    q, pool, table, cu, lens = _inputs([300, 5], [1000, 2000], 14, 2, 128, 64)
+    want = lib.paged_attention(q, pool, table, cu, lens, 300, 2000, 14, 0.088)
+    assert torch.equal(lib.paged_attention(q, pool, table, cu, lens, 300, 2000, 14, 0.088, out=q), want) and torch.equal(q, want)
+
+
+def test_refusals_of_the_wrapper():
+    q, pool, table, cu, lens = _inputs([2, 3], [40, 50], 4, 2, 64, 16)
+    call = lambda **kw: lib.paged_attention(*[kw.get(k, v) for k, v in dict(q=q, pool=pool, table=table, cu=cu, lens=lens).items()], 3, 50, kw.get("hq", 4), 0.1, out=kw.get("out"))  # noqa: E731
+    call()
+    for bad in (dict(q=q.float()), dict(q=q[:, :-64]), dict(pool=pool.half()), dict(pool=pool[:, :1]), dict(pool=pool.transpose(2, 3)), dict(table=table.long()), dict(table=table[0]),
+                dict(cu=cu[:-1]), dict(cu=cu.long()), dict(lens=lens[:1]), dict(out=torch.empty(5, 256, device="cuda")), dict(hq=3), dict(q=q.cpu()),
+                dict(out=torch.empty(5, 260, device="cuda", dtype=BF)[:, :256])):
+        with pytest.raises(lib.OmcError):
+            call(**bad)
+
+
 def test_two_streams_at_once():
     cases = [_inputs([n], [c], 14, 2, 128, 64, seed=i) for i, (n, c) in enumerate([(3, 5000), (40, 3000)])]
     alone = [lib.paged_attention(*x, m, 5000, 14, 0.088) for x, m in zip(cases, (3, 40))]

@@ -58,10 +58,21 @@ def _attend(L, **kw):
                                         (dict(pages=1 << 24), -2, "2^31"), (dict(n_seq=-1), -2, "negative"), (dict(max_new=-1), -2, "negative"), (dict(scale=0.0), -1, "scale"),
                                         (dict(scale=-0.1), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(q=P + 2), -3, "16-byte"),
                                         (dict(out=P + 8), -3, "16-byte"), (dict(ldq=516), -3, "multiples of 8"), (dict(ldq=504), -2, "overlap"), (dict(cu=None), -1, "null"),
-                                        (dict(table=None), -1, "null")])
+                                        (dict(table=None), -1, "null"), (dict(T=1 << 20, max_new=1 << 20, max_ctx=1 << 30), -2, "2^31 products"),
+                                        (dict(T=1 << 20, max_new=1 << 30), -2, "2^31 rows"), (dict(max_ctx=(1 << 30) + 1), -2, "2^30"),
+                                        (dict(max_ctx=100000), -1, "workspace"), (dict(max_ctx=100000, ws=P, wsb=1000), -1, "workspace"),
+                                        (dict(max_ctx=100000, ws=P + 8, wsb=1 << 40), -1, "workspace")])
 def test_attention(L, kw, rc, word):
     assert _attend(L, **kw) == rc and word in _said(L)
     assert _attend(L, T=0) == 0 and _attend(L, n_seq=0) == 0 and _attend(L, max_new=0) == 0
+
+
+def test_workspace_bytes(L):
+    size = lambda *a: L.omc_paged_chunk_attn_workspace_bytes(*a)  # noqa: E731
+    assert size(1, 1, 300, 28, 4, 128) == 0 < size(1, 1, 4096, 28, 4, 128)   # nothing is cut: nothing is joined
+    assert size(1, 1, 4096, 28, 4, 128) < 1 << 24 and size(1, 1, 4096, 28, 4, 96) < 0 and "64 or 128" in _said(L)
+    assert L.omc_wait_failed() == 0
+    lib.check_waits()
 
 
 def test_host_tensors_are_refused():
