@@ -30,14 +30,13 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "chunk_attention.cuh"
 #include "omc_internal.h"
 #include "sm100_step.cuh"
 
 namespace omc {
 
-typedef __nv_bfloat16 bf16;
-
-constexpr int kCaRows = 128, kCaKeys = 64, kCaBlock = 256, kCaThreads = 512;
+constexpr int kCaRows = 128, kCaBlock = 256, kCaThreads = 512;
 constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
 // Products (128 rows x 64 keys) a CTA has at least where blocks are cut: one of each stream. A single token behind 1087 positions, replayed: 16.4 us with 8, 13.1 with 2,
 // 12.1 with 1, which a token behind 2000 loses again (14.4 against 12.3).
@@ -48,25 +47,6 @@ constexpr int kCaJoinThreads = 256;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
 static __device__ unsigned int g_chunk_failures;   // waits that ran out
-
-struct ChunkArgs {
-  const bf16* q;
-  long long ldq;
-  const bf16* pool;        // [n_pages][2][Hkv][page_size][D]
-  const int32_t* table;    // [n_seq][max_pages]
-  const int32_t* cu;       // [n_seq + 1]
-  const int32_t* ctx;      // [n_seq]
-  bf16* out;
-  long long ldo;
-  int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, Hq, Hkv;
-  float scale_log2;
-  int wide;                // out is on 32-byte boundaries, its rows too
-  int4* head;              // workspace: [CTAs] (parts of the block that is cut behind this CTA or 0, first row of q, first row of the block, rows | key/value head << 16)
-  float2* ml;              // [2 CTAs][part_rows] maximum (base 2, scaled) and sum
-  float4* part;            // [2 CTAs][D / 4][part_rows]: the threads of a warp have neighbouring rows
-  int part_rows;
-  unsigned int* failed;
-};
 
 // A sequence as the kernel takes it: what the host promised is also a bound.
 struct CaSeq {
@@ -111,14 +91,6 @@ struct CaShape {
 
 // ---------------------------------------------------------------------------------------------------- the line of work and its parts
 __device__ __forceinline__ int ca_warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
-__device__ __forceinline__ int ca_warp_scan(int v, int lane) {   // inclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += up;
-  }
-  return v;
-}
 __device__ __forceinline__ CaSeq ca_shfl(const CaSeq& q, int from) {
   CaSeq r;
   r.base = __shfl_sync(0xffffffffu, q.base, from);
@@ -289,20 +261,9 @@ template <int N>
 __device__ __forceinline__ void ca_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 template <int N>
 __device__ __forceinline__ void ca_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
-__device__ __forceinline__ float ca_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // A whole sector: neighbouring threads have rows far apart, and 16 bytes at a time cost an SM as much of its way to L2.
 __device__ __forceinline__ void ca_store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
-// The maximum keeps a NaN, which then is the row's reference.
-__device__ __forceinline__ float ca_max3(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 __device__ __forceinline__ uint64_t ca_f2(float a, float b) {
   uint64_t r;
@@ -737,14 +698,10 @@ __global__ void __launch_bounds__(kCaJoinThreads, AHEAD > 4 ? 1 : 4) chunk_attn_
 }
 
 // ---------------------------------------------------------------------------------------------------- host
-struct CaPlan {
-  int grid, part_rows;
-  bool cut, fits;          // whether a block can be cut; whether the products can be counted in 31 bits
-  long long bytes;
-};
 static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
   const long long rows = (long long)max_new * (Hq / Hkv), tiles = max_ctx <= kCaKeys ? 1 : ((long long)max_ctx + kCaKeys - 1) / kCaKeys;
   const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * tiles, blocks = (long long)n_seq * Hkv * ((rows + kCaBlock - 1) / kCaBlock);
+  if (few_takes(rows, head_dim)) return few_plan(n_seq, Hkv, rows, tiles, head_dim);
   CaPlan p;
   p.fits = most < (1ll << 31);
   p.cut = tiles * (rows > kCaRows ? 2 : 1) > kCaWhole;
@@ -761,7 +718,8 @@ template <int D>
 static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   const int dev = cur_device();
-  if (!done[dev]) {
+  const bool few = few_takes((long long)a.max_new * (a.Hq / a.Hkv), D);
+  if (!few && !done[dev]) {
     cudaFuncAttributes at;
     cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D>);
     if (e == cudaSuccess && at.numRegs * 4 < kCaRegsLoad + 2 * kCaRegsSoftmax + kCaRegsIssue)
@@ -770,8 +728,8 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
     if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
     done[dev] = true;
   }
-  chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
-  int rc = check_launch("omc_paged_chunk_attn");
+  if (!few) chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
+  const int rc = few ? few_launch(a, D, plan.grid, st) : check_launch("omc_paged_chunk_attn");
   if (rc != OMC_OK || !plan.cut) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(plan.grid, (plan.part_rows * (D / 8) + kCaJoinThreads - 1) / kCaJoinThreads);
@@ -835,7 +793,9 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
   ChunkArgs a{};
   a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.pool = static_cast<const bf16*>(kv_pool); a.table = block_table; a.cu = cu_new; a.ctx = ctx_lens;
   a.out = static_cast<bf16*>(out); a.ldo = ldo; a.n_seq = n_seq; a.T = T; a.max_new = max_new; a.max_ctx = reach < max_ctx ? (int)reach : max_ctx;
-  a.n_pages = n_pages; a.max_pages = max_pages; a.page_size = page_size; a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * 1.4426950408889634f;
+  a.n_pages = n_pages; a.max_pages = max_pages; a.page_size = page_size;
+  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned int)page_size) : -1;
+  a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * 1.4426950408889634f;
   a.wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && ldo % 16 == 0;
   if (plan.bytes > 0) {
     a.head = static_cast<int4*>(workspace);

@@ -1,0 +1,453 @@
+// Attention over the paged cache for the few rows of a step of single or drafted tokens: what chunk_attention.cu computes, for sequences whose rows (token,
+// query head of the group) are no more than a tile or two of mma.sync has.
+//
+// Every key and value is read once and meets few rows, so HBM bounds a large call and the way from the launch to the first scores a small one. Neither wants
+// tcgen05: an M of 128 for 7 rows, a CTA's tensor memory and the hand-offs between its warps were 12 us of a call that reads 2 MB (this kernel: 9.7).
+// Here a warp is a pipeline of its own: it copies groups of 16 keys (32 of heads of 64) by cp.async into its ring of sub-slots (keys, values, keys, ...), takes the scores
+// from them with the rows' fragments in registers, keeps a maximum, a sum and an output of its own, and waits for nobody. The warps of a CTA take the groups of
+// its part of the line in turn and are merged where a block ends.
+#include <math.h>
+#include <stdint.h>
+
+#include "chunk_attention.cuh"
+#include "omc_internal.h"
+
+namespace omc {
+
+constexpr int kFewMinUnits = 2, kFewWhole = 8;
+
+template <int D, int MT>
+struct FewShape {
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kGroup = D == 128 ? 16 : 32, kPair = 32 / kGroup, kSub = kGroup * D * 2, kSubs = 4, kPitch = D + 8;
+  static constexpr int kRing = kWarps * kSubs * kSub, kQueries = MT * 16 * D * 2, kJoint = kWarps * 16 * kPitch * 4;
+  static constexpr int kSmem = kRing + kQueries + kJoint + kWarps * 16 * 8;
+  static constexpr int kPerSM = 2;
+  static_assert(kPerSM * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
+};
+
+// A sequence of the line, and what of it a CTA has: tiles [t0, t1) of a key/value head.
+struct FewWalk {
+  int seq, kvh, t0, t1;
+  int base, n, sees, keys, tiles;   // first row of q, tokens, keys that the first token sees (may be negative), keys that the last one sees, their tiles
+  int last_seq, last_kvh, last_tile;   // where the CTA's part ends (a tile of 0: in front of that block)
+  __device__ __forceinline__ void load(const ChunkArgs& a) {
+    base = a.cu[seq];
+    const int n_all = a.cu[seq + 1] - base, ctx = max(0, min(a.ctx[seq], a.max_ctx));
+    n = base < 0 ? 0 : max(0, min(min(n_all, a.max_new), a.T - base));
+    sees = ctx - n_all + 1;
+    keys = max(0, min(ctx, ctx - n_all + n));
+    tiles = max(1, (keys + kCaKeys - 1) / kCaKeys);
+  }
+  __device__ __forceinline__ bool enter(const ChunkArgs& a, int tile) {
+    const bool last = seq == last_seq && kvh == last_kvh;
+    t0 = tile;
+    t1 = last ? last_tile : tiles;
+    return t1 > t0;
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs& a) {
+    if (seq == last_seq && kvh == last_kvh) return false;
+    if (++kvh == a.Hkv) {
+      kvh = 0;
+      do {
+        if (++seq >= a.n_seq) return false;
+        load(a);
+      } while (n == 0);
+    }
+    return enter(a, 0);
+  }
+  __device__ __forceinline__ int groups(int per) const { return (max(0, min(keys, t1 * kCaKeys) - t0 * kCaKeys) + per - 1) / per; }
+};
+
+// The parts of the line: units (tiles, or blocks where none is cut) are counted by sequences, a lane has `per_lane` neighbouring ones.
+__device__ __forceinline__ int few_units(const ChunkArgs& a, int s) {   // of a block of sequence s
+  if (s >= a.n_seq) return 0;
+  FewWalk w;
+  w.seq = s;
+  w.load(a);
+  return w.n == 0 ? 0 : (a.head != nullptr ? w.tiles : 1);
+}
+struct FewPlace {
+  int seq, kvh, within, per;   // within, per: units of the block in front of the place, and all of them
+};
+// units: of a block of the lane's last sequence; upto: of the line with the lane's sequences; mine: of those.
+__device__ __forceinline__ FewPlace few_locate(const ChunkArgs& a, int u, int per_lane, int units, int upto, int mine, int lane) {
+  const unsigned int hit = __ballot_sync(0xffffffffu, u < upto);
+  if (hit == 0) return FewPlace{a.n_seq, 0, 0, 1};
+  const int from = __ffs(hit) - 1;
+  int start = __shfl_sync(0xffffffffu, upto - mine, from), per = __shfl_sync(0xffffffffu, units, from), seq = from;
+  if (per_lane > 1) {
+    seq *= per_lane;
+    for (int i = 0; i < per_lane; i += 32) {
+      const int own = i + lane < per_lane ? few_units(a, seq + i + lane) : 0, up = start + ca_warp_scan(own * a.Hkv, lane);
+      const unsigned int in = __ballot_sync(0xffffffffu, u < up);
+      if (in != 0) {
+        const int l = __ffs(in) - 1;
+        start = __shfl_sync(0xffffffffu, up - own * a.Hkv, l);
+        per = __shfl_sync(0xffffffffu, own, l);
+        seq += i + l;
+        break;
+      }
+      start = __shfl_sync(0xffffffffu, up, 31);
+    }
+  }
+  const int kvh = a.Hkv <= 32 ? __popc(__ballot_sync(0xffffffffu, lane + 1 < a.Hkv && u - start >= (lane + 1) * per)) : (u - start) / per;
+  return FewPlace{seq, kvh, u - start - kvh * per, per};
+}
+
+__device__ __forceinline__ float few_quad_max(float v) {
+  v = ca_max3(v, __shfl_xor_sync(0xffffffffu, v, 1), v);
+  return ca_max3(v, __shfl_xor_sync(0xffffffffu, v, 2), v);
+}
+__device__ __forceinline__ float few_quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <int D, int MT>
+__global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kPerSM) chunk_attn_few_kernel(const ChunkArgs a) {
+  using C = FewShape<D, MT>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.Hq / a.Hkv, cta = blockIdx.x;
+  pdl_launch();
+  // ------------------------------------------------------------------------------------------------ the CTA's part, found by every warp for itself
+  FewWalk w;
+  int first_tile;
+  {
+    const int per_lane = (a.n_seq + 31) >> 5;
+    int mine = 0, units = 0;
+    for (int i = 0; i < per_lane; ++i) {
+      units = few_units(a, lane * per_lane + i);
+      mine += units * a.Hkv;
+    }
+    const int upto = ca_warp_scan(mine, lane), total = __shfl_sync(0xffffffffu, upto, 31);
+    const int parts = min((int)gridDim.x, max(1, a.head != nullptr ? total / kFewMinUnits : total)), each = total / parts, more = total - each * parts;
+    auto cut = [&](int c) { return each * c + min(more, c); };
+    if (cta >= parts || total == 0) {
+      if (a.head != nullptr && tid == 0) a.head[cta] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    const int u0 = cut(cta), u1 = cut(cta + 1);
+    const FewPlace begin = few_locate(a, u0, per_lane, units, upto, mine, lane), end = few_locate(a, u1, per_lane, units, upto, mine, lane);
+    const bool cuts = a.head != nullptr;
+    w.seq = begin.seq;
+    w.kvh = begin.kvh;
+    first_tile = cuts ? begin.within : 0;
+    w.last_seq = end.seq;
+    w.last_kvh = end.kvh;
+    w.last_tile = cuts ? end.within : 0;
+    if (cuts && warp == 0) {
+      int4 head = make_int4(0, 0, 0, 0);
+      if (end.within > 0 && u0 <= u1 - end.within) {       // the block that is cut behind this CTA begins in it
+        const int closes = u1 - end.within + end.per;
+        for (int j0 = cta + 1; j0 < parts; j0 += 32) {
+          const unsigned int closed = __ballot_sync(0xffffffffu, j0 + lane < parts && cut(j0 + lane + 1) >= closes);
+          if (closed != 0) {
+            head.x = j0 + __ffs(closed) - cta;
+            break;
+          }
+        }
+        FewWalk q;
+        q.seq = end.seq;
+        q.load(a);
+        head.y = q.base;
+        head.w = q.n * rep | end.kvh << 16;
+      }
+      if (lane == 0) a.head[cta] = head;
+    }
+  }
+  w.load(a);
+  bool more = w.enter(a, first_tile);
+
+  // ------------------------------------------------------------------------------------------------ the warp's copies
+  uint8_t* const ring = smem + warp * (C::kSubs * C::kSub);
+  FewWalk wl = w;                                          // runs ahead of w
+  int lj = warp;
+  bool l_more = more;
+  // Rows of the pool by pairs of groups, one row per lane, looked up a pair ahead.
+  int page_next = -1, off_next = 0, left_next = 0, row = -1, left = 0, half = 0;
+  auto look_up = [&]() {
+    left_next = 0;
+    page_next = -1;
+    while (l_more && lj >= wl.groups(C::kGroup)) {
+      l_more = wl.next(a);
+      lj = warp;
+    }
+    if (!l_more) return;
+    const int ng = wl.groups(C::kGroup), g = lj + lane / C::kGroup * C::kWarps, key = wl.t0 * kCaKeys + g * C::kGroup + lane % C::kGroup;
+    if (g < ng && key < wl.keys) {
+      const int slot = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+      off_next = wl.kvh * a.page_size + key - slot * a.page_size;
+      page_next = a.table[(long long)wl.seq * a.max_pages + slot];
+    }
+    left_next = C::kPair == 1 || lj + C::kWarps >= ng ? 1 : 2;
+    lj += C::kPair * C::kWarps;
+  };
+  const int value_rows = a.Hkv * a.page_size;
+  constexpr int kLanes = D / 8, kRowsAt = 32 / kLanes;     // lanes of a row, rows of an instruction
+  const int c = lane % kLanes, sub_row = lane / kLanes;
+  int fill = 0;                                            // sub-slot of the next copy: keys in the even ones
+  auto copy = [&]() {
+    const bool values = fill & 1;
+    if (!values) {
+      if (left == 0) {
+        row = (unsigned int)page_next < (unsigned int)a.n_pages ? page_next * 2 * value_rows + off_next : -1;
+        left = left_next;
+        half = 0;
+        look_up();
+      }
+    }
+    if (left > 0) {
+      uint8_t* const dst = ring + fill * C::kSub;
+#pragma unroll
+      for (int i = 0; i < C::kGroup / kRowsAt; ++i) {
+        const int r = i * kRowsAt + sub_row, from = __shfl_sync(0xffffffffu, row, half * 16 + r);
+        const long long at = (long long)(max(from, 0) + (values && from >= 0 ? value_rows : 0)) * D + c * 8;
+        cp_async16(dst + r * (D * 2) + ((c ^ (r & 7)) << 4), a.pool + at, from >= 0);
+      }
+      if (values) {
+        --left;
+        ++half;
+      }
+    }
+    cp_async_commit();
+    fill = (fill + 1) % C::kSubs;
+  };
+  // The rows' queries, 16 bytes a thread at a time.
+  uint8_t* const queries = smem + C::kRing;
+  auto copy_queries = [&]() {
+    const int rows = w.n * rep;
+    for (int id = tid; id < MT * 16 * kLanes; id += C::kThreads) {
+      const int r = id / kLanes, token = w.n == 1 ? 0 : r / rep;
+      const bool there = r < rows;
+      cp_async16(queries + r * (D * 2) + ((c ^ (r & 7)) << 4), a.q + (there ? (long long)(w.base + token) * a.ldq + (long long)(w.kvh * rep + r - token * rep) * D + c * 8 : 0), there);
+    }
+    cp_async_commit();
+  };
+  if (more) copy_queries();
+  look_up();
+#pragma unroll 1
+  for (int i = 0; i < C::kSubs; ++i) copy();
+
+  // ------------------------------------------------------------------------------------------------ blocks
+  const uint32_t ring_at = smem_u32(ring);
+  float* const joint = reinterpret_cast<float*>(smem + C::kRing + C::kQueries);   // [warps][16][pitch], then maxima and sums [warps][16]
+  float2* const joint_ml = reinterpret_cast<float2*>(smem + C::kRing + C::kQueries + C::kJoint);
+  const float sl2 = a.scale_log2;
+  int use = 0;                                             // sub-slot of the next keys
+  cp_async_wait<C::kSubs>();                               // the queries
+  __syncthreads();
+  while (more) {
+    const int rows = w.n * rep, ng = w.groups(C::kGroup);
+    uint32_t qf[MT][D / 16][4];
+    int limit[MT][2];                                      // keys that the lane's rows see
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int r = t * 16 + (lane & 15);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        ldmatrix_x4(smem_u32(queries) + r * (D * 2) + (((2 * k + (lane >> 4)) ^ (r & 7)) << 4), qf[t][k][0], qf[t][k][1], qf[t][k][2], qf[t][k][3]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) limit[t][i] = min(w.keys, w.sees + (w.n == 1 ? 0 : (t * 16 + i * 8 + lane / 4) / rep));
+    }
+    float o[MT][D / 8][4], top[MT][2], sum[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      top[t][0] = top[t][1] = -INFINITY;
+      sum[t][0] = sum[t][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    }
+#pragma unroll 1
+    for (int g = warp; g < ng; g += C::kWarps) {
+      const int key0 = w.t0 * kCaKeys + g * C::kGroup;
+      // ---- scores
+      float s[MT][C::kGroup / 8][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < C::kGroup / 8; ++i) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+      cp_async_wait<C::kSubs - 1>();
+      __syncwarp();
+      {
+        const uint32_t at = ring_at + use * C::kSub;
+        const int r = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < C::kGroup / 16; ++j) {
+            uint32_t b[4];
+            ldmatrix_x4(at + (j * 16 + r) * (D * 2) + (((2 * k + (lane >> 3 & 1)) ^ (r & 7)) << 4), b[0], b[1], b[2], b[3]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              mma_bf16_16816(s[t][2 * j], qf[t][k], b[0], b[1]);
+              mma_bf16_16816(s[t][2 * j + 1], qf[t][k], b[2], b[3]);
+            }
+          }
+      }
+      __syncwarp();
+      copy();
+      // ---- softmax
+      uint32_t p[MT][C::kGroup / 16][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (key0 + C::kGroup > w.sees) {                   // the first token does not see all
+#pragma unroll
+          for (int i = 0; i < C::kGroup / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + i * 8 + (lane % 4) * 2 + (e & 1) >= limit[t][e >> 1]) s[t][i][e] = -INFINITY;
+        }
+        float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < C::kGroup / 8; ++i) {
+          most[0] = ca_max3(most[0], s[t][i][0], s[t][i][1]);
+          most[1] = ca_max3(most[1], s[t][i][2], s[t][i][3]);
+        }
+        most[0] = few_quad_max(most[0]) * sl2;
+        most[1] = few_quad_max(most[1]) * sl2;
+        // the reference moves where it would be passed by 2^8, and to a NaN
+        if (__any_sync(0xffffffffu, !(most[0] <= top[t][0] + 8.f) || !(most[1] <= top[t][1] + 8.f)) ) {
+          float f[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float now = ca_max3(top[t][i], most[i], most[i]);
+            f[i] = top[t][i] == -INFINITY ? 0.f : ca_ex2(top[t][i] - now);
+            top[t][i] = now;
+            sum[t][i] *= f[i];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[t][i][0] *= f[0];
+            o[t][i][1] *= f[0];
+            o[t][i][2] *= f[1];
+            o[t][i][3] *= f[1];
+          }
+        }
+        const float neg[2] = {top[t][0] == -INFINITY ? 0.f : -top[t][0], top[t][1] == -INFINITY ? 0.f : -top[t][1]};
+#pragma unroll
+        for (int i = 0; i < C::kGroup / 8; ++i) {
+          float e[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) e[x] = ca_ex2(fmaf(s[t][i][x], sl2, neg[x >> 1]));
+          sum[t][0] += e[0] + e[1];
+          sum[t][1] += e[2] + e[3];
+          // probabilities up to 2^8, rounded to bf16 for the product: half a step each whatever their size
+          p[t][i / 2][(i & 1) * 2] = pack_bf16(e[0], e[1]);
+          p[t][i / 2][(i & 1) * 2 + 1] = pack_bf16(e[2], e[3]);
+        }
+      }
+      // ---- output
+      cp_async_wait<C::kSubs - 1>();
+      __syncwarp();
+      {
+        const uint32_t at = ring_at + (use + 1) * C::kSub;
+        const int r = lane & 15;
+#pragma unroll
+        for (int j = 0; j < C::kGroup / 16; ++j)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(at + (j * 16 + r) * (D * 2) + (((2 * i + (lane >> 4)) ^ (r & 7)) << 4), b[0], b[1], b[2], b[3]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              mma_bf16_16816(o[t][2 * i], p[t][j], b[0], b[1]);
+              mma_bf16_16816(o[t][2 * i + 1], p[t][j], b[2], b[3]);
+            }
+          }
+      }
+      __syncwarp();
+      copy();
+      use = (use + 2) % C::kSubs;
+    }
+    // ------------------------------------------------------------------------------------------------ the warps' parts together, 16 rows at a time
+    const bool finished = a.head == nullptr || (w.t0 == 0 && w.t1 == w.tiles), single = w.n == 1;
+    const long long part = 2ll * cta + (w.t0 == 0 ? 1 : 0);
+    bf16* const to = a.out + (long long)w.base * a.ldo + (long long)(w.kvh * rep) * D;
+    more = w.next(a);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (t * 16 >= rows) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 8 + lane / 4;
+        const float l = few_quad_sum(sum[t][i]);
+        if (lane % 4 == 0) joint_ml[warp * 16 + r] = make_float2(top[t][i], l);
+        if (t * 16 + r < rows && warp < ng) {
+          float* const dst = joint + (warp * 16 + r) * C::kPitch + (lane % 4) * 2;
+#pragma unroll
+          for (int k = 0; k < D / 8; ++k) *reinterpret_cast<float2*>(dst + k * 8) = make_float2(o[t][k][2 * i], o[t][k][2 * i + 1]);
+        }
+      }
+      __syncthreads();
+      if (t == 0 && more) copy_queries();                  // every warp has its fragments of the last ones
+      for (int id = tid; id < min(16, rows - t * 16) * (D / 4); id += C::kThreads) {
+        const int r = id / (D / 4), d4 = id % (D / 4), at = t * 16 + r;
+        float2 ml[C::kWarps];
+        float most = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < C::kWarps; ++k) {
+          ml[k] = joint_ml[k * 16 + r];
+          most = ca_max3(most, ml[k].x, ml[k].x);
+        }
+#pragma unroll
+        for (int k = 0; k < C::kWarps; ++k) {
+          if (ml[k].x == -INFINITY) continue;              // a warp without keys, or whose keys the row does not see
+          const float f = ca_ex2(ml[k].x - most);
+          const float4 v = *reinterpret_cast<const float4*>(joint + (k * 16 + r) * C::kPitch + d4 * 4);
+          l += f * ml[k].y;
+          acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+        }
+        if (finished) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const int token = single ? 0 : at / rep;
+          *reinterpret_cast<uint2*>(to + (long long)token * a.ldo + (at - token * rep) * D + d4 * 4) =
+              make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+        } else {
+          a.part[(part * (D / 4) + d4) * a.part_rows + at] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (d4 == 0) a.ml[part * a.part_rows + at] = make_float2(most, l);
+        }
+      }
+      if (t == 0) cp_async_wait<0>();                      // the queries; what of the ring is under way has been so for as long
+      __syncthreads();
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+bool few_takes(long long rows, int head_dim) { return rows * head_dim <= 4096; }
+
+CaPlan few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim) {
+  const long long blocks = (long long)n_seq * Hkv, most = blocks * tiles;
+  const int slots = 2 * num_sms();
+  CaPlan p;
+  p.fits = most < (1ll << 31);
+  p.cut = tiles > kFewWhole;
+  const long long parts = p.cut ? most / kFewMinUnits : blocks;
+  p.grid = parts < 1 ? 1 : (parts < slots ? (int)parts : slots);
+  p.cut = p.cut && p.grid > 1;
+  p.part_rows = (int)rows;
+  p.bytes = p.cut ? (long long)p.grid * 16 + 2ll * p.grid * p.part_rows * (8 + 4ll * head_dim) : 0;
+  return p;
+}
+
+template <int D, int MT>
+static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  const int dev = cur_device();
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, MT>::kSmem);
+    if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  chunk_attn_few_kernel<D, MT><<<grid, FewShape<D, MT>::kThreads, FewShape<D, MT>::kSmem, st>>>(a);
+  return check_launch("omc_paged_chunk_attn");
+}
+
+int few_launch(const ChunkArgs& a, int head_dim, int grid, cudaStream_t st) {
+  const int rows = a.max_new * (a.Hq / a.Hkv);
+  if (head_dim == 128) return rows <= 16 ? launch<128, 1>(a, grid, st) : launch<128, 2>(a, grid, st);
+  return rows <= 16 ? launch<64, 1>(a, grid, st) : rows <= 32 ? launch<64, 2>(a, grid, st) : rows <= 48 ? launch<64, 3>(a, grid, st) : launch<64, 4>(a, grid, st);
+}
+
+}  // namespace omc
