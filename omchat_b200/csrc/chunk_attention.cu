@@ -8,7 +8,7 @@
 //   two streams of 128 rows take turns on the tensor pipe: S = Q K^T into TMEM, softmax in registers (a thread per row, running maximum and sum), P back to
 //   TMEM over its scores as bf16, O += P V with P as the operand in tensor memory. Scores go into two buffers per stream: a
 //   product is 256 to 400 cycles of the pipe and 330 more until who waits for it goes on, so the next scores are made while these are in their softmax.
-//   A block of at most 128 rows (all of a step of single tokens) gives its one tile of queries to both streams, which take every other tile of keys and are
+//   A block of at most 128 rows (a few drafted tokens) gives its one tile of queries to both streams, which take every other tile of keys and are
 //   merged at the end: the rows of a stream lie on the same lanes of TMEM.
 // One CTA per SM walks over its share of the work: the products of all blocks (128 rows x 64 keys) in one line, cut into equal parts whatever the
 // lengths are, at a tile of keys. Each CTA finds its part from cu and ctx by itself. A block that is cut leaves its parts (unnormalised O, maximum, sum; two at
@@ -18,11 +18,12 @@
 //   warps 12, 13  MMA issuers of the two streams (one thread each: a thread's waits and its products, which are taken one after the other, would hold up the
 //                 other stream's)
 //   warps 14, 15  queries
+// Calls of few rows a block go to chunk_attention_few.cu.
 // Keys behind a block's last are zero-filled, so what a page holds behind a context meets no product.
 //
 // Measured (28 heads on 4 of 128, pages of 64): 2048 rows behind 28672 positions 719 us = 1210 TFLOP/s in a short run, 0.72 of a cuBLAS burst, and 832 us = 1050
-// TFLOP/s back to back under the power limit; 4 x 2048 rows behind 600 to 2048: 252 us; 512 behind 4096: 51 us; 32 single tokens behind up to 4096: 45 us, 5.8 TB/s of keys and
-// values while the line lasts; one behind 1087: 12.8 us. Many rows are bound by a tile's chain (1830 cycles for 256 rows: scores read 140, maximum 230,
+// TFLOP/s back to back under the power limit; 4 x 2048 rows behind 600 to 2048: 252 us; 512 behind 4096: 51 us; 32 x 4 (28 rows a block) behind up to
+// 4096: 44 us, of 175 MB of keys and values. Many rows are bound by a tile's chain (1830 cycles for 256 rows: scores read 140, maximum 230,
 // exponentials 830 of which the exponential unit takes 512, waits for scores 300) with the tensor pipe at some 1300 of them, 768 of which are S at the rate
 // of shared memory (128 bytes a cycle: with 64 keys to a product two thirds of what it reads are queries). Few rows are bound by HBM, after 4 us until a CTA's first scores. A block's end
 // costs 8 000 cycles (64 KB out, 64 KB of queries in, at some 46 bytes a cycle and SM), a cut 128 KB of parts on top of that, written and read.
@@ -701,8 +702,10 @@ __global__ void __launch_bounds__(kCaJoinThreads, AHEAD > 4 ? 1 : 4) chunk_attn_
 static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int head_dim) {
   const long long rows = (long long)max_new * (Hq / Hkv), tiles = max_ctx <= kCaKeys ? 1 : ((long long)max_ctx + kCaKeys - 1) / kCaKeys;
   const long long most = (long long)n_seq * Hkv * ((rows + kCaRows - 1) / kCaRows) * tiles, blocks = (long long)n_seq * Hkv * ((rows + kCaBlock - 1) / kCaBlock);
-  if (few_takes(rows, head_dim)) return few_plan(n_seq, Hkv, rows, tiles, head_dim);
   CaPlan p;
+  if (few_plan(n_seq, Hkv, rows, tiles, head_dim, p)) return p;
+  p.few = false;
+  p.cluster = 0;
   p.fits = most < (1ll << 31);
   p.cut = tiles * (rows > kCaRows ? 2 : 1) > kCaWhole;
   const long long parts = p.cut ? most / kCaMinUnits : blocks;
@@ -715,22 +718,7 @@ static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int 
 }
 
 template <int D>
-static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
-  static bool done[kMaxDevices] = {};
-  const int dev = cur_device();
-  const bool few = few_takes((long long)a.max_new * (a.Hq / a.Hkv), D);
-  if (!few && !done[dev]) {
-    cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D>);
-    if (e == cudaSuccess && at.numRegs * 4 < kCaRegsLoad + 2 * kCaRegsSoftmax + kCaRegsIssue)
-      return set_error(OMC_ERR_CUDA, "omc_paged_chunk_attn: built with fewer registers than its warps divide");
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, CaShape<D>::kSmem);
-    if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
-    done[dev] = true;
-  }
-  if (!few) chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
-  const int rc = few ? few_launch(a, D, plan.grid, st) : check_launch("omc_paged_chunk_attn");
-  if (rc != OMC_OK || !plan.cut) return rc;
+static int ca_join(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(plan.grid, (plan.part_rows * (D / 8) + kCaJoinThreads - 1) / kCaJoinThreads);
   cfg.blockDim = dim3(kCaJoinThreads);
@@ -744,6 +732,28 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   const cudaError_t e = plan.part_rows <= 64 ? cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 8>, a) : cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 3>, a);
   if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");
+}
+
+int chunk_join(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st) {
+  return head_dim == 64 ? ca_join<64>(a, plan, st) : ca_join<128>(a, plan, st);
+}
+
+template <int D>
+static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  const int dev = cur_device();
+  if (!done[dev]) {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D>);
+    if (e == cudaSuccess && at.numRegs * 4 < kCaRegsLoad + 2 * kCaRegsSoftmax + kCaRegsIssue)
+      return set_error(OMC_ERR_CUDA, "omc_paged_chunk_attn: built with fewer registers than its warps divide");
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, CaShape<D>::kSmem);
+    if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
+  const int rc = check_launch("omc_paged_chunk_attn");
+  return rc != OMC_OK || !plan.cut ? rc : ca_join<D>(a, plan, st);
 }
 
 }  // namespace omc
@@ -794,6 +804,7 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
   a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.pool = static_cast<const bf16*>(kv_pool); a.table = block_table; a.cu = cu_new; a.ctx = ctx_lens;
   a.out = static_cast<bf16*>(out); a.ldo = ldo; a.n_seq = n_seq; a.T = T; a.max_new = max_new; a.max_ctx = reach < max_ctx ? (int)reach : max_ctx;
   a.n_pages = n_pages; a.max_pages = max_pages; a.page_size = page_size;
+  a.cluster = plan.cluster;
   a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned int)page_size) : -1;
   a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * 1.4426950408889634f;
   a.wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && ldo % 16 == 0;
@@ -803,6 +814,7 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
     a.part = reinterpret_cast<float4*>(a.ml + 2ll * plan.grid * plan.part_rows);
     a.part_rows = plan.part_rows;
   }
+  if (plan.few) return few_launch(a, plan, head_dim, (cudaStream_t)stream);
   rc = step_failure_word(&a.failed);
   if (rc != OMC_OK) return rc;
   return head_dim == 64 ? ca_launch<64>(a, plan, (cudaStream_t)stream) : ca_launch<128>(a, plan, (cudaStream_t)stream);

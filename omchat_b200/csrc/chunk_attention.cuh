@@ -20,7 +20,7 @@ struct ChunkArgs {
   const int32_t* ctx;      // [n_seq]
   bf16* out;
   long long ldo;
-  int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, page_shift, Hq, Hkv;
+  int n_seq, T, max_new, max_ctx, n_pages, max_pages, page_size, page_shift, cluster, Hq, Hkv;
   float scale_log2;
   int wide;                // out is on 32-byte boundaries, its rows too
   int4* head;              // workspace: [CTAs] (parts of the block that is cut behind this CTA or 0, first row of q, first row of the block, rows | key/value head << 16)
@@ -31,14 +31,16 @@ struct ChunkArgs {
 };
 
 struct CaPlan {
-  int grid, part_rows;
+  int grid, part_rows, cluster;   // cluster: of few rows, CTAs that share a block; 0: the line is cut
+  bool few;                // chunk_attention_few.cu has it
   bool cut, fits;          // whether a block can be cut; whether the products can be counted in 31 bits
   long long bytes;
 };
-// Few rows: whether a call is one, how it is cut, and its launch (without that of the kernel that joins the parts).
-bool few_takes(long long rows, int head_dim);
-CaPlan few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim);
-int few_launch(const ChunkArgs& a, int head_dim, int grid, cudaStream_t st);
+// Few rows: whether the call is one, with its plan, and the launches.
+bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim, CaPlan& p);
+int few_launch(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st);
+// Joins the parts of blocks that were cut (chunk_attention.cu).
+int chunk_join(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st);
 
 __device__ __forceinline__ int ca_warp_scan(int v, int lane) {   // inclusive
 #pragma unroll

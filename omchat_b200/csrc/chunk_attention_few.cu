@@ -1,11 +1,21 @@
-// Attention over the paged cache for the few rows of a step of single or drafted tokens: what chunk_attention.cu computes, for sequences whose rows (token,
-// query head of the group) are no more than a tile or two of mma.sync has.
+// Attention over the paged cache for the few rows of a step of single or drafted tokens: what chunk_attention.cu computes, where the rows (token, query head of
+// the group) of a sequence and key/value head fit one to three tiles of mma.sync.
 //
-// Every key and value is read once and meets few rows, so HBM bounds a large call and the way from the launch to the first scores a small one. Neither wants
-// tcgen05: an M of 128 for 7 rows, a CTA's tensor memory and the hand-offs between its warps were 12 us of a call that reads 2 MB (this kernel: 9.7).
-// Here a warp is a pipeline of its own: it copies groups of 16 keys (32 of heads of 64) by cp.async into its ring of sub-slots (keys, values, keys, ...), takes the scores
-// from them with the rows' fragments in registers, keeps a maximum, a sum and an output of its own, and waits for nobody. The warps of a CTA take the groups of
-// its part of the line in turn and are merged where a block ends.
+// Every key and value is read once and meets few rows, so HBM bounds a large call, and a small one the way from the launch to the first scores. Neither wants
+// tcgen05: for 7 rows an M of 128, tensor memory and the hand-offs between warps cost 12.9 us of a token behind 1087 positions (28 heads on 4 of 128, 2 MB; this kernel 8.0) and 42
+// of 32 tokens behind up to 4096 (175 MB; 34.9, of which 27 at the rate of a copy; all in a graph).
+//
+// Here a warp is a pipeline of its own and waits for nobody: it copies groups of 16 keys (32 of heads of 64) by cp.async into a ring of its own (keys, values, keys, values: 4 KB
+// each), takes the scores with the rows in registers, keeps a maximum, a sum and an output, and the warps of a CTA take the groups of a block in turn. Two CTAs of four
+// warps per SM have 128 KB under way (an SM takes in some 46 bytes a cycle: 1.4 thousand cycles' worth). Where a block ends the warps are merged.
+//
+// Who has which keys: a block (a sequence's rows of one key/value head) is a cluster's of up to 8 CTAs, which join their parts through each other's shared memory: one launch, no
+// workspace, and no search for a CTA's share. Where that leaves CTAs more than eight tiles of 64 keys (long contexts, or more blocks than fill the GPU evenly) all
+// products lie in one line that is cut evenly, as in chunk_attention.cu, and a second kernel joins: 1 token behind 8000 20.6 us by clusters, 11.7 cut; 32 behind 4096 39.7 and 34.9;
+// 64 behind 2000 37.2 and 35.6; but 8 behind 2000 10.1 and 12.6, one behind 1087 8.0 and 9.7.
+//
+// What a small call is made of (one token behind 1087, cycles): lengths 700, page of the first rows 900, copies 1400 (shared memory's way in), a group 1100 (scores 370, softmax 290,
+// output 330) of up to three per warp, merging 1500 and joining 1300.
 #include <math.h>
 #include <stdint.h>
 
@@ -14,7 +24,8 @@
 
 namespace omc {
 
-constexpr int kFewMinUnits = 2, kFewWhole = 8;
+// Tiles that a CTA has at least where blocks are cut (one token behind 8000: 11.7 us with 2, 12.1 with 3, 12.9 with 4); CTAs of a cluster; tiles per CTA up to which clusters share.
+constexpr int kFewMinUnits = 2, kFewCluster = 8, kFewTiles = 8;
 
 template <int D, int MT>
 struct FewShape {
@@ -64,7 +75,7 @@ __device__ __forceinline__ int few_units(const ChunkArgs& a, int s) {   // of a 
   FewWalk w;
   w.seq = s;
   w.load(a);
-  return w.n == 0 ? 0 : (a.head != nullptr ? w.tiles : 1);
+  return w.n == 0 ? 0 : w.tiles;
 }
 struct FewPlace {
   int seq, kvh, within, per;   // within, per: units of the block in front of the place, and all of them
@@ -103,7 +114,24 @@ __device__ __forceinline__ float few_quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-template <int D, int MT>
+__device__ __forceinline__ uint32_t few_mapa(uint32_t at, uint32_t cta) {   // the address in the shared memory of another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ float2 few_remote2(uint32_t at, uint32_t cta) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(few_mapa(at, cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 few_remote4(uint32_t at, uint32_t cta) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(few_mapa(at, cta)) : "memory");
+  return v;
+}
+
+// kShared: a block is one CTA's or that of a cluster, whose parts are joined through shared memory; else the line is cut.
+template <int D, int MT, bool kShared>
 __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kPerSM) chunk_attn_few_kernel(const ChunkArgs a) {
   using C = FewShape<D, MT>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -112,7 +140,17 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
   // ------------------------------------------------------------------------------------------------ the CTA's part, found by every warp for itself
   FewWalk w;
   int first_tile;
-  {
+  if constexpr (kShared) {
+    w.seq = cta / (a.Hkv * a.cluster);
+    w.kvh = cta / a.cluster - w.seq * a.Hkv;
+    w.load(a);
+    if (w.n == 0) return;                                  // all CTAs of the cluster
+    const int rank = cta & (a.cluster - 1);
+    first_tile = w.tiles * rank / a.cluster;
+    w.last_seq = w.seq;
+    w.last_kvh = w.kvh;
+    w.last_tile = w.tiles * (rank + 1) / a.cluster;
+  } else {
     const int per_lane = (a.n_seq + 31) >> 5;
     int mine = 0, units = 0;
     for (int i = 0; i < per_lane; ++i) {
@@ -120,22 +158,21 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
       mine += units * a.Hkv;
     }
     const int upto = ca_warp_scan(mine, lane), total = __shfl_sync(0xffffffffu, upto, 31);
-    const int parts = min((int)gridDim.x, max(1, a.head != nullptr ? total / kFewMinUnits : total)), each = total / parts, more = total - each * parts;
+    const int parts = min((int)gridDim.x, max(1, total / kFewMinUnits)), each = total / parts, more = total - each * parts;
     auto cut = [&](int c) { return each * c + min(more, c); };
     if (cta >= parts || total == 0) {
-      if (a.head != nullptr && tid == 0) a.head[cta] = make_int4(0, 0, 0, 0);
+      if (tid == 0) a.head[cta] = make_int4(0, 0, 0, 0);
       return;
     }
     const int u0 = cut(cta), u1 = cut(cta + 1);
     const FewPlace begin = few_locate(a, u0, per_lane, units, upto, mine, lane), end = few_locate(a, u1, per_lane, units, upto, mine, lane);
-    const bool cuts = a.head != nullptr;
     w.seq = begin.seq;
     w.kvh = begin.kvh;
-    first_tile = cuts ? begin.within : 0;
+    first_tile = begin.within;
     w.last_seq = end.seq;
     w.last_kvh = end.kvh;
-    w.last_tile = cuts ? end.within : 0;
-    if (cuts && warp == 0) {
+    w.last_tile = end.within;
+    if (warp == 0) {
       int4 head = make_int4(0, 0, 0, 0);
       if (end.within > 0 && u0 <= u1 - end.within) {       // the block that is cut behind this CTA begins in it
         const int closes = u1 - end.within + end.per;
@@ -154,9 +191,9 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
       }
       if (lane == 0) a.head[cta] = head;
     }
+    w.load(a);
   }
-  w.load(a);
-  bool more = w.enter(a, first_tile);
+  bool more = w.enter(a, first_tile) || kShared;          // a CTA of a cluster without tiles has its part in the joining
 
   // ------------------------------------------------------------------------------------------------ the warp's copies
   uint8_t* const ring = smem + warp * (C::kSubs * C::kSub);
@@ -233,6 +270,12 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
   float* const joint = reinterpret_cast<float*>(smem + C::kRing + C::kQueries);   // [warps][16][pitch], then maxima and sums [warps][16]
   float2* const joint_ml = reinterpret_cast<float2*>(smem + C::kRing + C::kQueries + C::kJoint);
   const float sl2 = a.scale_log2;
+  auto store = [&](bf16* to, int at, bool single, int d4, const float (&acc)[4], float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int token = single ? 0 : at / rep;
+    *reinterpret_cast<uint2*>(to + (long long)token * a.ldo + (at - token * rep) * D + d4 * 4) =
+        make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+  };
   int use = 0;                                             // sub-slot of the next keys
   cp_async_wait<C::kSubs>();                               // the queries
   __syncthreads();
@@ -360,7 +403,7 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
       use = (use + 2) % C::kSubs;
     }
     // ------------------------------------------------------------------------------------------------ the warps' parts together, 16 rows at a time
-    const bool finished = a.head == nullptr || (w.t0 == 0 && w.t1 == w.tiles), single = w.n == 1;
+    const bool finished = w.t0 == 0 && w.t1 == w.tiles, single = w.n == 1;
     const long long part = 2ll * cta + (w.t0 == 0 ? 1 : 0);
     bf16* const to = a.out + (long long)w.base * a.ldo + (long long)(w.kvh * rep) * D;
     more = w.next(a);
@@ -397,57 +440,200 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
           l += f * ml[k].y;
           acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
         }
-        if (finished) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int token = single ? 0 : at / rep;
-          *reinterpret_cast<uint2*>(to + (long long)token * a.ldo + (at - token * rep) * D + d4 * 4) =
-              make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+        if (kShared && a.cluster > 1) {
+          *reinterpret_cast<float4*>(smem + (at * D + d4 * 4) * 4) = make_float4(acc[0], acc[1], acc[2], acc[3]);   // the ring has been read
+          if (d4 == 0) *reinterpret_cast<float2*>(smem + MT * 16 * D * 4 + at * 8) = make_float2(most, l);
+        } else if (finished) {
+          store(to, at, single, d4, acc, l);
         } else {
           a.part[(part * (D / 4) + d4) * a.part_rows + at] = make_float4(acc[0], acc[1], acc[2], acc[3]);
           if (d4 == 0) a.ml[part * a.part_rows + at] = make_float2(most, l);
         }
       }
       if (t == 0) cp_async_wait<0>();                      // the queries; what of the ring is under way has been so for as long
-      __syncthreads();
+      if (more || t + 1 < MT) __syncthreads();
+    }
+    if (kShared && a.cluster > 1) {
+      __syncwarp();
+      cluster_sync_all();
+      for (int id = (int)cluster_ctarank() * C::kThreads + tid; id < rows * (D / 4); id += a.cluster * C::kThreads) {
+        const int at = id / (D / 4), d4 = id % (D / 4);
+        float2 ml[kFewCluster];
+        float4 v[kFewCluster];
+#pragma unroll
+        for (int k = 0; k < kFewCluster; ++k) {
+          const uint32_t from = min(k, a.cluster - 1);
+          ml[k] = few_remote2(smem_u32(smem + MT * 16 * D * 4 + at * 8), from);
+          v[k] = few_remote4(smem_u32(smem + (at * D + d4 * 4) * 4), from);
+          if (k >= a.cluster) ml[k].x = -INFINITY;
+        }
+        float most = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kFewCluster; ++k) most = ca_max3(most, ml[k].x, ml[k].x);
+#pragma unroll
+        for (int k = 0; k < kFewCluster; ++k) {
+          if (ml[k].x == -INFINITY) continue;
+          const float f = ca_ex2(ml[k].x - most);
+          l += f * ml[k].y;
+          acc[0] += f * v[k].x, acc[1] += f * v[k].y, acc[2] += f * v[k].z, acc[3] += f * v[k].w;
+        }
+        store(to, at, single, d4, acc, l);
+      }
+      __syncwarp();
+      cluster_sync_all();                                  // nobody leaves before its parts have been read
     }
   }
   cp_async_wait<0>();
 }
 
-// ---------------------------------------------------------------------------------------------------- host
-bool few_takes(long long rows, int head_dim) { return rows * head_dim <= 4096; }
+// Joins blocks that were cut into many parts: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A CTA has 32 dimensions, and its
+// threads share the parts too: one token behind 8000 positions, 63 parts: 11.7 us against 16.9 where a thread has all parts of its dimensions. With few parts that other
+// kernel's fewer CTAs win: 32 tokens behind 4096, two or three parts: 34.9 against 39.7.
+constexpr int kFewManyParts = 16, kFewJoinThreads = 256, kFewSlices = 16, kFewAhead = 8;
 
-CaPlan few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim) {
-  const long long blocks = (long long)n_seq * Hkv, most = blocks * tiles;
-  const int slots = 2 * num_sms();
-  CaPlan p;
-  p.fits = most < (1ll << 31);
-  p.cut = tiles > kFewWhole;
-  const long long parts = p.cut ? most / kFewMinUnits : blocks;
-  p.grid = parts < 1 ? 1 : (parts < slots ? (int)parts : slots);
-  p.cut = p.cut && p.grid > 1;
-  p.part_rows = (int)rows;
-  p.bytes = p.cut ? (long long)p.grid * 16 + 2ll * p.grid * p.part_rows * (8 + 4ll * head_dim) : 0;
-  return p;
+template <int D>
+__global__ void __launch_bounds__(kFewJoinThreads) chunk_attn_few_join_kernel(const ChunkArgs a) {
+  __shared__ float sums[10][kFewJoinThreads];
+  pdl_wait();
+  const int i = blockIdx.x, rep = a.Hq / a.Hkv, tid = threadIdx.x;
+  const int4 head = a.head[i];
+  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16;
+  if (parts == 0) return;
+  const int items = rows * 4, slices = min(kFewSlices, kFewJoinThreads / items), slice = tid / items, item = tid - slice * items, group = item / rows, row = item - group * rows;
+  const int d8 = blockIdx.y * 4 + group;
+  float top = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto take = [&](float m, float sum, const float (&v)[8]) {   // m is not below -inf and not above `top`
+    if (m == -INFINITY) return;                              // no part, or one in which the row saw no key
+    const float f = ca_ex2(m - top);
+    l += f * sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += f * v[e];
+  };
+  auto raise = [&](float most) {
+    const float f = top == -INFINITY ? 0.f : ca_ex2(top - most);
+    top = most;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= f;
+  };
+  if (slice < slices) {
+    for (int k0 = slice; k0 < parts; k0 += slices * kFewAhead) {
+      float2 m[kFewAhead];
+      float4 u[kFewAhead], v[kFewAhead];
+#pragma unroll
+      for (int k = 0; k < kFewAhead; ++k) {
+        const int p = k0 + k * slices;
+        const long long part = 2ll * (i + min(p, parts - 1)) + (p == 0 ? 1 : 0);
+        m[k] = a.ml[part * a.part_rows + row];
+        u[k] = a.part[(part * (D / 4) + 2 * d8) * a.part_rows + row];
+        v[k] = a.part[(part * (D / 4) + 2 * d8 + 1) * a.part_rows + row];
+        if (p >= parts) m[k].x = -INFINITY;
+      }
+      float most = top;
+#pragma unroll
+      for (int k = 0; k < kFewAhead; ++k) most = ca_max3(most, m[k].x, m[k].x);
+      raise(most);
+#pragma unroll
+      for (int k = 0; k < kFewAhead; ++k) {
+        const float w[8] = {u[k].x, u[k].y, u[k].z, u[k].w, v[k].x, v[k].y, v[k].z, v[k].w};
+        take(m[k].x, m[k].y, w);
+      }
+    }
+    sums[0][tid] = top;
+    sums[1][tid] = l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[2 + e][tid] = acc[e];
+  }
+  __syncthreads();
+  if (slice > 0) return;
+  float most = top;
+  for (int s = 1; s < slices; ++s) most = ca_max3(most, sums[0][s * items + item], most);
+  raise(most);
+  for (int s = 1; s < slices; ++s) {
+    const int at = s * items + item;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = sums[2 + e][at];
+    take(sums[0][at], sums[1][at], w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int token = row / rep, h = row - token * rep;
+  *reinterpret_cast<uint4*>(a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + d8 * 8) =
+      make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv), pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
 }
 
-template <int D, int MT>
+// ---------------------------------------------------------------------------------------------------- host
+// More than a tile of rows only pays in the cluster form: the lanes hold the output of all rows. Heads of 128: 64 x 4 tokens (28 rows) behind 600 24.8 us against 29.0 on tcgen05, 8 x 4 behind
+// 3000 18.8 and 19.2, but cut 32 x 4 behind 4096 54.8 and 44.2. Heads of 64: 8 x 5 (35 rows) behind 1531 10.7 and 13.3, 8 x 7 (49) behind 3000 22.5 and 15.0.
+bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim, CaPlan& p) {
+  if (rows * head_dim > 4096 || rows > 48) return false;
+  const long long blocks = (long long)n_seq * Hkv, most = blocks * tiles;
+  const int slots = 2 * num_sms();
+  p.fits = most < (1ll << 31);
+  p.few = true;
+  p.part_rows = (int)rows;
+  p.cluster = 1;
+  while (p.cluster < kFewCluster && p.cluster < tiles && blocks * p.cluster * 2 <= slots) p.cluster *= 2;
+  p.cut = tiles > kFewTiles * p.cluster + kFewTiles / 2;
+  if (p.cut && rows * head_dim > 2048) return false;
+  if (p.cut) p.cluster = 0;
+  const long long parts = p.cut ? most / kFewMinUnits : blocks * p.cluster;
+  p.grid = p.cut ? (int)(parts < 1 ? 1 : parts < slots ? parts : slots) : (int)parts;
+  p.bytes = p.cut ? (long long)p.grid * 16 + 2ll * p.grid * p.part_rows * (8 + 4ll * head_dim) : 0;
+  return true;
+}
+
+template <int D, int MT, bool kShared>
 static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   const int dev = cur_device();
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, MT>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_few_kernel<D, MT, kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, MT>::kSmem);
     if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
     done[dev] = true;
   }
-  chunk_attn_few_kernel<D, MT><<<grid, FewShape<D, MT>::kThreads, FewShape<D, MT>::kSmem, st>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(FewShape<D, MT>::kThreads);
+  cfg.dynamicSmemBytes = FewShape<D, MT>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kShared && a.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_kernel<D, MT, kShared>, a);
+  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");
 }
 
-int few_launch(const ChunkArgs& a, int head_dim, int grid, cudaStream_t st) {
-  const int rows = a.max_new * (a.Hq / a.Hkv);
-  if (head_dim == 128) return rows <= 16 ? launch<128, 1>(a, grid, st) : launch<128, 2>(a, grid, st);
-  return rows <= 16 ? launch<64, 1>(a, grid, st) : rows <= 32 ? launch<64, 2>(a, grid, st) : rows <= 48 ? launch<64, 3>(a, grid, st) : launch<64, 4>(a, grid, st);
+template <int D>
+static int few_join(const ChunkArgs& a, int grid, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, D / 32);
+  cfg.blockDim = dim3(kFewJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_join_kernel<D>, a);
+  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+  return check_launch("omc_paged_chunk_attn");
+}
+
+int few_launch(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st) {
+  const int rows = plan.part_rows, grid = plan.grid;
+  if (a.cluster > 0) {
+    if (head_dim == 128) return rows <= 16 ? launch<128, 1, true>(a, grid, st) : launch<128, 2, true>(a, grid, st);
+    return rows <= 16 ? launch<64, 1, true>(a, grid, st) : rows <= 32 ? launch<64, 2, true>(a, grid, st) : launch<64, 3, true>(a, grid, st);
+  }
+  const int rc = head_dim == 128 ? launch<128, 1, false>(a, grid, st) : rows <= 16 ? launch<64, 1, false>(a, grid, st) : launch<64, 2, false>(a, grid, st);
+  if (rc != OMC_OK) return rc;
+  if ((long long)a.n_seq * a.Hkv * kFewManyParts > grid) return chunk_join(a, plan, head_dim, st);
+  return head_dim == 128 ? few_join<128>(a, grid, st) : few_join<64>(a, grid, st);
 }
 
 }  // namespace omc

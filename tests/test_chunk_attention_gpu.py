@@ -34,6 +34,10 @@ def _check(out, q, pool, table, new, ctx, hq, hkv, head, scale):
     for s, (n, c) in enumerate(zip(new, ctx)):
         if n == 0:
             continue
+        if c == 0:
+            assert not out[first:first + n].any()
+            first += n
+            continue
         k, v = pool[table[s].long()].double().permute(1, 2, 0, 3, 4).reshape(2, hkv, -1, head)[:, :, :c]
         rows = q[first:first + n].double().view(n, hkv, hq // hkv, head)
         seen = torch.arange(c, device="cuda")[None] <= (c - n + torch.arange(n, device="cuda"))[:, None]
@@ -176,6 +180,37 @@ def test_many_sequences():
     q, pool, table, cu, lens = _inputs(new, ctx, 14, 2, 64, 16)
     out = lib.paged_attention(q, pool, table, cu, lens, 60, 3000, 14, 0.125)
     _check(out, q, pool, table, new, ctx, 14, 2, 64, 0.125)
+
+
+FEW = [  # calls of few rows a sequence and head: blocks that clusters share, of any number of tiles, and the line that is cut
+    ([1, 0, 1, 1], [0, 5, 1, 64], 14, 2, 128, 64), ([4, 2], [2, 90], 14, 2, 64, 16), ([1, 1], [3000, 200], 40, 40, 64, 16), ([5] * 8, [100 * i + 5 for i in range(8)], 14, 2, 64, 16),
+    ([4, 1, 3], [700, 2000, 5], 28, 4, 128, 24), ([1] * 60 + [0] * 30 + [1] * 60, [(i * 37) % 3000 + 1 for i in range(150)], 14, 2, 128, 64),
+    ([1] * 1100, [800 if i == 700 else i % 90 + 1 for i in range(1100)], 3, 1, 64, 64), ([1], [20000], 4, 4, 64, 64), ([2, 1], [16000, 9], 14, 2, 64, 128), ([1] * 70, [999] * 70, 16, 2, 128, 64),
+    ([4] * 40, [(i * 53) % 700 + 4 for i in range(40)], 28, 4, 128, 64), ([6, 6], [400, 77], 8, 1, 64, 64), ([1], [1500], 48, 1, 64, 64), ([1] * 3, [64 * 8, 64 * 8 + 1, 64 * 7], 4, 1, 128, 32),
+]
+
+
+@pytest.mark.parametrize("new,ctx,hq,hkv,head,page", FEW, ids=range(len(FEW)))
+def test_few_rows(new, ctx, hq, hkv, head, page):
+    q, pool, table, cu, lens = _inputs(new, ctx, hq, hkv, head, page, extra=2)
+    out = torch.full((q.shape[0], hq * head), 5.0, device="cuda", dtype=BF)
+    lib.paged_attention(q, pool, table, cu, lens, max(new), max(ctx), hq, head ** -0.5, out=out)
+    _check(out, q, pool, table, new, ctx, hq, hkv, head, head ** -0.5)
+    assert bool((out[sum(new):] == 5).all())
+    again = lib.paged_attention(q, pool, table, cu, lens, max(new), max(ctx), hq, head ** -0.5)
+    assert torch.equal(again[: sum(new)], out[: sum(new)])
+
+
+def test_few_rows_whose_numbers_are_not_finite():
+    """What no row sees stays out; a NaN among the keys of a token reaches its rows and, of the others, only rows of the same sequence and key/value head."""
+    new, ctx = [1, 2, 1], [200, 700, 3000]
+    q, pool, table, cu, lens = _inputs(new, ctx, 14, 2, 128, 64)
+    want = lib.paged_attention(q, pool, table, cu, lens, 2, 3000, 14, 0.088)
+    assert bool(want.isfinite().all())
+    pool[table[1, 3].long(), 0, 1, 5] = float("nan")
+    got = lib.paged_attention(q, pool, table, cu, lens, 2, 3000, 14, 0.088)
+    assert bool(got[1:3, 7 * 128:].isnan().all()) and torch.equal(got[1:3, : 7 * 128], want[1:3, : 7 * 128])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])
 
 
 def test_queries_and_results_in_the_same_rows():
