@@ -39,11 +39,11 @@ namespace omc {
 
 constexpr int kCaRows = 128, kCaBlock = 256, kCaThreads = 512;
 constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 columns of queries, of keys
-// Products (128 rows x 64 keys) a CTA has at least where blocks are cut: one of each stream. A single token behind 1087 positions, replayed: 16.4 us with 8, 13.1 with 2,
-// 12.1 with 1, which a token behind 2000 loses again (14.4 against 12.3).
+// Products (128 rows x 64 keys) a CTA has at least where blocks are cut: one of each stream. 8 tokens (56 rows) behind 600 positions: 16.8 us with 8, 14.4 with 4, 11.2 with 2,
+// 11.8 with 1, with which 8 behind 2000 take 15.9 instead of 13.0.
 constexpr int kCaMinUnits = 2;
-// Products of a block up to which none is cut and there is no second kernel: 10.5 us against 12.5 for a token behind 300 positions, 18 against 12.7 behind 900.
-constexpr int kCaWhole = 6;
+// Products of a block up to which none is cut and there is no second kernel: 8 tokens behind 400 positions (7) 11.4 us against 12.9, behind 300 10.1 and 12.7.
+constexpr int kCaWhole = 7;
 constexpr int kCaJoinThreads = 256;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
