@@ -20,7 +20,8 @@ constexpr int kRegs = 6, kFloats = 8, kStack = 34, kMaxArgs = kRegs + kStack;
 
 // Integers and pointers fill the six registers and then 8-byte stack slots in their order, floats the eight vector registers in theirs, however the two are mixed
 // in the prototype; slots behind the last argument are not read.
-typedef int (*Fn)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float, float, float, float, float, float, float, float, int64_t, int64_t, int64_t, int64_t, int64_t,
+// A result of 64 bits is the whole of a register, one of int its lower half.
+typedef int64_t (*Fn)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float, float, float, float, float, float, float, float, int64_t, int64_t, int64_t, int64_t, int64_t,
                   int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                   int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 
@@ -29,7 +30,7 @@ struct Entry {
   vectorcallfunc call;
   Fn fn;
   PyObject* other;   // the ctypes function: arguments of any other kind go to it
-  int n;
+  int n, wide;       // wide: the result is a long long
   char sig[kMaxArgs + 1];   // P pointer, I int, L long long, F float
 };
 
@@ -66,12 +67,12 @@ PyObject* entry_call(PyObject* self, PyObject* const* args, size_t nargsf, PyObj
   }
   for (; ni < kMaxArgs; ++ni) v[ni] = 0;
   {
-    int rc;
+    int64_t rc;
     Py_BEGIN_ALLOW_THREADS;
     rc = e->fn(v[0], v[1], v[2], v[3], v[4], v[5], f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7], v[6], v[7], v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15], v[16],
                v[17], v[18], v[19], v[20], v[21], v[22], v[23], v[24], v[25], v[26], v[27], v[28], v[29], v[30], v[31], v[32], v[33], v[34], v[35], v[36], v[37], v[38], v[39]);
     Py_END_ALLOW_THREADS;
-    return PyLong_FromLong(rc);
+    return PyLong_FromLongLong(e->wide ? rc : (int64_t)(int32_t)rc);
   }
 other:
   PyErr_Clear();
@@ -85,12 +86,13 @@ void entry_dealloc(PyObject* self) {
 
 PyTypeObject EntryType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// entry(address, signature, ctypes function) -> a callable, or None where the signature does not fit
+// entry(address, signature, ctypes function, result is a long long) -> a callable, or None where the signature does not fit
 PyObject* make_entry(PyObject*, PyObject* args) {
   unsigned long long address;
   const char* sig;
   PyObject* other;
-  if (!PyArg_ParseTuple(args, "KsO", &address, &sig, &other)) return nullptr;
+  int wide = 0;
+  if (!PyArg_ParseTuple(args, "KsO|p", &address, &sig, &other, &wide)) return nullptr;
   const size_t n = strlen(sig);
   int floats = 0;
   for (size_t i = 0; i < n; ++i) floats += sig[i] == 'F';
@@ -102,6 +104,7 @@ PyObject* make_entry(PyObject*, PyObject* args) {
   Py_INCREF(other);
   e->other = other;
   e->n = (int)n;
+  e->wide = wide;
   memcpy(e->sig, sig, n + 1);
   return reinterpret_cast<PyObject*>(e);
 }

@@ -586,8 +586,9 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, 
     n = turns.numel()
     _vector(turns, n, _F64, "rotary: turns")
     if out is None:
-        out = torch.empty_like(x)
-    ldy = _rows(out, T, heads * head_dim, dtype, "rotary: out")
+        out, ldy = x.new_empty((T, heads * head_dim)), heads * head_dim
+    else:
+        ldy = _rows(out, T, heads * head_dim, dtype, "rotary: out")
     rc = load().omc_rotary_rows(x, 0 if dtype is _BF16 else 1, ldx, pos, T, heads, head_dim, turns, 2 * n, 1 if halves else 0, 1 if back else 0, mscale, out, ldy,
                                 _stream())
     _check(rc, "omc_rotary_rows")
@@ -609,9 +610,11 @@ def rotary_kv_append(qkv: torch.Tensor, pos: torch.Tensor, seq_ids: Optional[tor
     n = turns.numel()
     _vector(turns, n, _F64, "rotary_kv_append: turns")
     if q_out is None:
-        q_out = qkv.new_empty((T, Hq * head))
+        q_out, ldq = qkv.new_empty((T, Hq * head)), Hq * head
+    else:
+        ldq = _rows(q_out, T, Hq * head, _BF16, "rotary_kv_append: q_out")
     rc = load().omc_rotary_kv_append(qkv, ld, pos, seq_ids, T, Hq, Hkv, head, turns, 2 * n, 1 if halves else 0, mscale, q_out,
-                                     _rows(q_out, T, Hq * head, _BF16, "rotary_kv_append: q_out"), kv_pool, n_pages, block_table, block_table.shape[0],
+                                     ldq, kv_pool, n_pages, block_table, block_table.shape[0],
                                      block_table.shape[1], page, _stream())
     _check(rc, "omc_rotary_kv_append")
     return q_out
@@ -630,12 +633,14 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
     _vector(cu_new, n_seq + 1, _I32, "paged_attention: cu_new")
     _vector(ctx_lens, n_seq, _I32, "paged_attention: ctx_lens")
     if out is None:
-        out = torch.empty_like(q)
+        out, ldo = q.new_empty((T, Hq * head)), Hq * head
+    else:
+        ldo = _rows(out, T, Hq * head, _BF16, "paged_attention: out")
     L = load()
     need = L.omc_paged_chunk_attn_workspace_bytes(n_seq, max_new, max_ctx, Hq, Hkv, head)
     ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None   # of this call alone: calls of other streams and graphs have their own
-    rc = L.omc_paged_chunk_attn(q, ldq, kv_pool, n_pages, block_table, max_pages, page, cu_new, ctx_lens, n_seq, T, max_new, max_ctx, Hq, Hkv, head, scale, out,
-                                _rows(out, T, Hq * head, _BF16, "paged_attention: out"), ws, need, _stream())
+    rc = L.omc_paged_chunk_attn(q, ldq, kv_pool, n_pages, block_table, max_pages, page, cu_new, ctx_lens, n_seq, T, max_new, max_ctx, Hq, Hkv, head, scale, out, ldo, ws, need,
+                                _stream())
     _check(rc, "omc_paged_chunk_attn")
     if ws is not None:
         add_launches(1)

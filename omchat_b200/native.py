@@ -59,8 +59,8 @@ class Entries:
             fn.restype = res
             fn.argtypes = [Pointer if a is c_void_p else a for a in args]
             entry = None
-            if native is not None and res is c_int and all(a in _KINDS for a in args):
-                entry = native.entry(ctypes.cast(fn, c_void_p).value, "".join(_KINDS[a] for a in args), fn)
+            if native is not None and res in (c_int, c_longlong) and all(a in _KINDS for a in args):
+                entry = native.entry(ctypes.cast(fn, c_void_p).value, "".join(_KINDS[a] for a in args), fn, res is c_longlong)
             setattr(self, name, fn if entry is None else entry)
 
     def __getattr__(self, name):

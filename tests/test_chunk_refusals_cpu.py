@@ -69,8 +69,8 @@ def test_attention(L, kw, rc, word):
 
 def test_workspace_bytes(L):
     size = lambda *a: L.omc_paged_chunk_attn_workspace_bytes(*a)  # noqa: E731
-    assert size(1, 1, 300, 28, 4, 128) == 0 < size(1, 1, 4096, 28, 4, 128)   # nothing is cut: nothing is joined
-    assert size(1, 1, 4096, 28, 4, 128) < 1 << 24 and size(1, 1, 4096, 28, 4, 96) < 0 and "64 or 128" in _said(L)
+    assert size(1, 1, 300, 28, 4, 128) == 0 < size(1, 1, 40960, 28, 4, 128)   # nothing is cut: nothing is joined
+    assert size(1, 1, 40960, 28, 4, 128) < 1 << 24 and size(1, 1, 4096, 28, 4, 96) < 0 and "64 or 128" in _said(L)
     assert L.omc_wait_failed() == 0
     lib.check_waits()
 
