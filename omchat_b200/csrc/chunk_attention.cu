@@ -31,6 +31,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "chunk_attention.cuh"
 #include "omc_internal.h"
 #include "sm100_step.cuh"
@@ -44,7 +46,7 @@ constexpr int kCaQBox = kCaRows * 128, kCaBox = kCaKeys * 128;   // bytes of 64 
 constexpr int kCaMinUnits = 2;
 // Products of a block up to which none is cut and there is no second kernel: 8 tokens behind 400 positions (7) 11.4 us against 12.9, behind 300 10.1 and 12.7.
 constexpr int kCaWhole = 7;
-constexpr int kCaJoinThreads = 256;
+constexpr int kCaManyParts = 9, kCaJoinThreads = 256;
 constexpr int kCaRegsLoad = 64, kCaRegsSoftmax = 192, kCaRegsIssue = 64;   // of the 4 x 128 a thread that the CTA is launched with
 
 static __device__ unsigned int g_chunk_failures;   // waits that ran out
@@ -651,47 +653,106 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   }
 }
 
-// The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A thread has eight dimensions of a
-// row, neighbouring threads neighbouring rows, AHEAD parts' loads under way together.
-template <int D, int AHEAD>
-__global__ void __launch_bounds__(kCaJoinThreads, AHEAD > 4 ? 1 : 4) chunk_attn_join_kernel(const ChunkArgs a) {
-  pdl_wait();
-  const int i = blockIdx.x, rep = a.Hq / a.Hkv;
-  const int4 head = a.head[i];
-  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16, id = blockIdx.y * kCaJoinThreads + threadIdx.x;
-  const int group = id / max(rows, 1), row = id - group * rows;
-  if (parts == 0 || group >= D / 8) return;
-  float top = -INFINITY, l = 0.f, acc[8];
+// The j-th of the CTAs that say that a block is cut behind them, with what they say; -1: there are fewer.
+__device__ __forceinline__ int ca_find_cut(const ChunkArgs& a, int from, int j, int tid, int4& head) {
+  __shared__ int4 found;
+  __shared__ int at, count[kCaJoinThreads / 32];
+  const int lane = tid & 31;
+  if (tid == 0) at = -1;
+  for (int c0 = 0, before = 0; c0 < from; c0 += kCaJoinThreads) {
+    const int4 mine = c0 + tid < from ? a.head[c0 + tid] : make_int4(0, 0, 0, 0);
+    const unsigned int cut = __ballot_sync(0xffffffffu, mine.x > 0);
+    if (lane == 0) count[tid >> 5] = __popc(cut);
+    __syncthreads();
+    int rank = before + __popc(cut & ((1u << lane) - 1u));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  for (int k0 = 0; k0 < parts; k0 += AHEAD) {
-    float2 m[AHEAD];
-    float4 u[AHEAD], v[AHEAD];
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const long long part = 2ll * (i + min(k0 + k, parts - 1)) + (k0 + k == 0 ? 1 : 0);
-      m[k] = a.ml[part * a.part_rows + row];
-      u[k] = a.part[(part * (D / 4) + 2 * group) * a.part_rows + row];
-      v[k] = a.part[(part * (D / 4) + 2 * group + 1) * a.part_rows + row];
-      if (k0 + k >= parts) m[k].x = -INFINITY;
+    for (int w = 0; w < kCaJoinThreads / 32; ++w) {
+      if (w < tid >> 5) rank += count[w];
+      before += count[w];
     }
-    float most = top;
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) most = ca_max3(most, m[k].x, most);
-    const float before = top == -INFINITY ? 0.f : ca_ex2(top - most);
+    if (mine.x > 0 && rank == j) {
+      found = mine;
+      at = c0 + tid;
+    }
+    __syncthreads();
+  }
+  head = found;
+  return at;
+}
+
+// The parts of a block that was cut: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. An item is eight dimensions of a row, neighbouring
+// threads have neighbouring rows, and AHEAD parts' loads of a thread are under way together. With few parts a block the CTAs of column i of the grid take what CTA i has to say.
+// With many (FIND) only few columns would have work: column j finds the j-th block that was cut, its CTAs take `per` items each, and `slices` threads share an item's parts: 4 tokens behind
+// 20000 positions 18.9 us against 22.3, 8 behind 4000 15.8 and 19.1, one behind 8000 12.1 and 16.9; but 8 behind 600, with five parts a block, 11.7 and 11.2.
+template <int D, int AHEAD, bool FIND>
+__global__ void __launch_bounds__(kCaJoinThreads, AHEAD > 4 ? 1 : 4) chunk_attn_join_kernel(const ChunkArgs a, int from, int per, int slices) {
+  const int tid = threadIdx.x, rep = a.Hq / a.Hkv;
+  pdl_wait();
+  int i = blockIdx.x;
+  int4 head;
+  if constexpr (FIND) {
+    i = ca_find_cut(a, from, i, tid, head);
+    if (i < 0) return;
+  } else {
+    head = a.head[i];
+  }
+  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16;
+  if (parts == 0) return;
+  const int slice = tid / per, item = tid - slice * per, id = blockIdx.y * per + item, group = id / rows, row = id - group * rows;
+  const bool works = slice < slices && group < D / 8;
+  float top = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto raise = [&](float most) {
+    const float f = top == -INFINITY ? 0.f : ca_ex2(top - most);
     top = most;
-    l *= before;
+    l *= f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] *= before;
+    for (int e = 0; e < 8; ++e) acc[e] *= f;
+  };
+  auto take = [&](float m, float sum, float4 u, float4 v) {  // m is at most `top`
+    if (m == -INFINITY) return;                              // no part, or one in which the row saw no key
+    const float f = ca_ex2(m - top);
+    l += f * sum;
+    acc[0] += f * u.x, acc[1] += f * u.y, acc[2] += f * u.z, acc[3] += f * u.w;
+    acc[4] += f * v.x, acc[5] += f * v.y, acc[6] += f * v.z, acc[7] += f * v.w;
+  };
+  if (works) {
+    for (int k0 = slice; k0 < parts; k0 += slices * AHEAD) {
+      float2 m[AHEAD];
+      float4 u[AHEAD], v[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (m[k].x == -INFINITY) continue;                 // no part, or one in which the row saw no key
-      const float f = ca_ex2(m[k].x - most);
-      l += f * m[k].y;
-      acc[0] += f * u[k].x, acc[1] += f * u[k].y, acc[2] += f * u[k].z, acc[3] += f * u[k].w;
-      acc[4] += f * v[k].x, acc[5] += f * v[k].y, acc[6] += f * v[k].z, acc[7] += f * v[k].w;
+      for (int k = 0; k < AHEAD; ++k) {
+        const int p = k0 + k * slices;
+        const long long part = 2ll * (i + min(p, parts - 1)) + (p == 0 ? 1 : 0);
+        m[k] = a.ml[part * a.part_rows + row];
+        u[k] = a.part[(part * (D / 4) + 2 * group) * a.part_rows + row];
+        v[k] = a.part[(part * (D / 4) + 2 * group + 1) * a.part_rows + row];
+        if (p >= parts) m[k].x = -INFINITY;
+      }
+      float most = top;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) most = ca_max3(most, m[k].x, most);
+      raise(most);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) take(m[k].x, m[k].y, u[k], v[k]);
     }
   }
+  if (FIND && slices > 1) {
+    __shared__ float sums[10][kCaJoinThreads];
+    sums[0][tid] = top;
+    sums[1][tid] = l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[2 + e][tid] = acc[e];
+    __syncthreads();
+    if (slice > 0 || !works) return;
+    float most = top;
+    for (int s = 1; s < slices; ++s) most = ca_max3(most, sums[0][s * per + item], most);
+    raise(most);
+    for (int s = 1; s < slices; ++s) {
+      const int at = s * per + item;
+      take(sums[0][at], sums[1][at], make_float4(sums[2][at], sums[3][at], sums[4][at], sums[5][at]), make_float4(sums[6][at], sums[7][at], sums[8][at], sums[9][at]));
+    }
+  }
+  if (!works) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int token = (head.z + row) / rep, h = head.z + row - token * rep;
   *reinterpret_cast<uint4*>(a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + group * 8) =
@@ -705,6 +766,7 @@ static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int 
   CaPlan p;
   if (few_plan(n_seq, Hkv, rows, tiles, head_dim, p)) return p;
   p.few = false;
+  p.blocks = blocks;
   p.cluster = 0;
   p.fits = most < (1ll << 31);
   p.cut = tiles * (rows > kCaRows ? 2 : 1) > kCaWhole;
@@ -719,8 +781,12 @@ static CaPlan ca_plan(int n_seq, int max_new, int max_ctx, int Hq, int Hkv, int 
 
 template <int D>
 static int ca_join(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
+  const bool find = plan.blocks * kCaManyParts < plan.grid;
+  const int columns = find ? (int)plan.blocks : plan.grid, items = plan.part_rows * (D / 8), parts = find ? plan.grid / columns + 1 : 3, full = find ? 4 * num_sms() : 0;
+  const int least = (items + kCaJoinThreads - 1) / kCaJoinThreads, wish = std::min(full / columns, items / 32);
+  const int per = (items + std::max(least, wish) - 1) / std::max(least, wish), slices = find ? std::min(std::min(kCaJoinThreads / per, 16), parts) : 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(plan.grid, (plan.part_rows * (D / 8) + kCaJoinThreads - 1) / kCaJoinThreads);
+  cfg.gridDim = dim3(columns, (items + per - 1) / per);
   cfg.blockDim = dim3(kCaJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -728,8 +794,9 @@ static int ca_join(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // few rows are cut into many parts; many rows into two or three, and need the registers for threads (512 rows behind 4096: 54 us against 57 with eight)
-  const cudaError_t e = plan.part_rows <= 64 ? cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 8>, a) : cudaLaunchKernelEx(&cfg, chunk_attn_join_kernel<D, 3>, a);
+  const bool ahead = find ? parts > 3 * slices : plan.part_rows <= 64;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, find ? (ahead ? chunk_attn_join_kernel<D, 8, true> : chunk_attn_join_kernel<D, 3, true>) : (ahead ? chunk_attn_join_kernel<D, 8, false> : chunk_attn_join_kernel<D, 3, false>),
+                                           a, plan.grid, per, slices);
   if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");
 }

@@ -34,7 +34,7 @@ struct CaPlan {
   int grid, part_rows, cluster;   // cluster: of few rows, CTAs that share a block; 0: the line is cut
   bool few;                // chunk_attention_few.cu has it
   bool cut, fits;          // whether a block can be cut; whether the products can be counted in 31 bits
-  long long bytes;
+  long long blocks, bytes; // at most as many blocks; of the workspace
 };
 // Few rows: whether the call is one, with its plan, and the launches.
 bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim, CaPlan& p);

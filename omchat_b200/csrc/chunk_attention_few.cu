@@ -486,82 +486,6 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
   cp_async_wait<0>();
 }
 
-// Joins blocks that were cut into many parts: the first is the second one that CTA i left, the others the first ones of the CTAs behind it. A CTA has 32 dimensions, and its
-// threads share the parts too: one token behind 8000 positions, 63 parts: 11.7 us against 16.9 where a thread has all parts of its dimensions. With few parts that other
-// kernel's fewer CTAs win: 32 tokens behind 4096, two or three parts: 34.9 against 39.7.
-constexpr int kFewManyParts = 16, kFewJoinThreads = 256, kFewSlices = 16, kFewAhead = 8;
-
-template <int D>
-__global__ void __launch_bounds__(kFewJoinThreads) chunk_attn_few_join_kernel(const ChunkArgs a) {
-  __shared__ float sums[10][kFewJoinThreads];
-  pdl_wait();
-  const int i = blockIdx.x, rep = a.Hq / a.Hkv, tid = threadIdx.x;
-  const int4 head = a.head[i];
-  const int parts = head.x, rows = head.w & 0xffff, kvh = head.w >> 16;
-  if (parts == 0) return;
-  const int items = rows * 4, slices = min(kFewSlices, kFewJoinThreads / items), slice = tid / items, item = tid - slice * items, group = item / rows, row = item - group * rows;
-  const int d8 = blockIdx.y * 4 + group;
-  float top = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto take = [&](float m, float sum, const float (&v)[8]) {   // m is not below -inf and not above `top`
-    if (m == -INFINITY) return;                              // no part, or one in which the row saw no key
-    const float f = ca_ex2(m - top);
-    l += f * sum;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += f * v[e];
-  };
-  auto raise = [&](float most) {
-    const float f = top == -INFINITY ? 0.f : ca_ex2(top - most);
-    top = most;
-    l *= f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] *= f;
-  };
-  if (slice < slices) {
-    for (int k0 = slice; k0 < parts; k0 += slices * kFewAhead) {
-      float2 m[kFewAhead];
-      float4 u[kFewAhead], v[kFewAhead];
-#pragma unroll
-      for (int k = 0; k < kFewAhead; ++k) {
-        const int p = k0 + k * slices;
-        const long long part = 2ll * (i + min(p, parts - 1)) + (p == 0 ? 1 : 0);
-        m[k] = a.ml[part * a.part_rows + row];
-        u[k] = a.part[(part * (D / 4) + 2 * d8) * a.part_rows + row];
-        v[k] = a.part[(part * (D / 4) + 2 * d8 + 1) * a.part_rows + row];
-        if (p >= parts) m[k].x = -INFINITY;
-      }
-      float most = top;
-#pragma unroll
-      for (int k = 0; k < kFewAhead; ++k) most = ca_max3(most, m[k].x, m[k].x);
-      raise(most);
-#pragma unroll
-      for (int k = 0; k < kFewAhead; ++k) {
-        const float w[8] = {u[k].x, u[k].y, u[k].z, u[k].w, v[k].x, v[k].y, v[k].z, v[k].w};
-        take(m[k].x, m[k].y, w);
-      }
-    }
-    sums[0][tid] = top;
-    sums[1][tid] = l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sums[2 + e][tid] = acc[e];
-  }
-  __syncthreads();
-  if (slice > 0) return;
-  float most = top;
-  for (int s = 1; s < slices; ++s) most = ca_max3(most, sums[0][s * items + item], most);
-  raise(most);
-  for (int s = 1; s < slices; ++s) {
-    const int at = s * items + item;
-    float w[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = sums[2 + e][at];
-    take(sums[0][at], sums[1][at], w);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int token = row / rep, h = row - token * rep;
-  *reinterpret_cast<uint4*>(a.out + (long long)(head.y + token) * a.ldo + (long long)(kvh * rep + h) * D + d8 * 8) =
-      make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv), pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
-}
-
 // ---------------------------------------------------------------------------------------------------- host
 // More than a tile of rows only pays in the cluster form: the lanes hold the output of all rows. Heads of 128: 64 x 4 tokens (28 rows) behind 600 24.8 us against 29.0 on tcgen05, 8 x 4 behind
 // 3000 18.8 and 19.2, but cut 32 x 4 behind 4096 54.8 and 44.2. Heads of 64: 8 x 5 (35 rows) behind 1531 10.7 and 13.3, 8 x 7 (49) behind 3000 22.5 and 15.0.
@@ -571,6 +495,7 @@ bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim,
   const int slots = 2 * num_sms();
   p.fits = most < (1ll << 31);
   p.few = true;
+  p.blocks = blocks;
   p.part_rows = (int)rows;
   p.cluster = 1;
   while (p.cluster < kFewCluster && p.cluster < tiles && blocks * p.cluster * 2 <= slots) p.cluster *= 2;
@@ -608,22 +533,6 @@ static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
   return check_launch("omc_paged_chunk_attn");
 }
 
-template <int D>
-static int few_join(const ChunkArgs& a, int grid, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, D / 32);
-  cfg.blockDim = dim3(kFewJoinThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_join_kernel<D>, a);
-  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
-  return check_launch("omc_paged_chunk_attn");
-}
-
 int few_launch(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st) {
   const int rows = plan.part_rows, grid = plan.grid;
   if (a.cluster > 0) {
@@ -631,9 +540,7 @@ int few_launch(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_
     return rows <= 16 ? launch<64, 1, true>(a, grid, st) : rows <= 32 ? launch<64, 2, true>(a, grid, st) : launch<64, 3, true>(a, grid, st);
   }
   const int rc = head_dim == 128 ? launch<128, 1, false>(a, grid, st) : rows <= 16 ? launch<64, 1, false>(a, grid, st) : launch<64, 2, false>(a, grid, st);
-  if (rc != OMC_OK) return rc;
-  if ((long long)a.n_seq * a.Hkv * kFewManyParts > grid) return chunk_join(a, plan, head_dim, st);
-  return head_dim == 128 ? few_join<128>(a, grid, st) : few_join<64>(a, grid, st);
+  return rc != OMC_OK ? rc : chunk_join(a, plan, head_dim, st);
 }
 
 }  // namespace omc
