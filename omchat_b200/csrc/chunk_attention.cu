@@ -27,7 +27,7 @@
 // exponentials 830 of which the exponential unit takes 512, waits for scores 300) with the tensor pipe at some 1300 of them, 768 of which are S at the rate
 // of shared memory (128 bytes a cycle: with 64 keys to a product two thirds of what it reads are queries). Few rows are bound by HBM, after 4 us until a CTA's first scores. A block's end
 // costs 8 000 cycles (64 KB out, 64 KB of queries in, at some 46 bytes a cycle and SM), a cut 128 KB of parts on top of that, written and read.
-// The order of sums goes by how the line is cut, that is by the lengths of all sequences of a call and the number of SMs; the same call has the same bits.
+// The order of sums goes by how the line is cut, that is by the lengths of all sequences of a call, its bounds of them and the number of SMs; the same call has the same bits.
 #include <math.h>
 #include <stdint.h>
 
@@ -881,8 +881,8 @@ extern "C" int omc_paged_chunk_attn(const void* q, long long ldq, const void* kv
     a.part = reinterpret_cast<float4*>(a.ml + 2ll * plan.grid * plan.part_rows);
     a.part_rows = plan.part_rows;
   }
-  if (plan.few) return few_launch(a, plan, head_dim, (cudaStream_t)stream);
   rc = step_failure_word(&a.failed);
   if (rc != OMC_OK) return rc;
+  if (plan.few) return few_launch(a, plan, head_dim, (cudaStream_t)stream);
   return head_dim == 64 ? ca_launch<64>(a, plan, (cudaStream_t)stream) : ca_launch<128>(a, plan, (cudaStream_t)stream);
 }

@@ -69,7 +69,7 @@ struct FewWalk {
   __device__ __forceinline__ int groups(int per) const { return (max(0, min(keys, t1 * kCaKeys) - t0 * kCaKeys) + per - 1) / per; }
 };
 
-// The parts of the line: units (tiles, or blocks where none is cut) are counted by sequences, a lane has `per_lane` neighbouring ones.
+// The parts of the line: its units are the tiles of all blocks, counted by sequences, of which a lane has `per_lane` neighbouring ones.
 __device__ __forceinline__ int few_units(const ChunkArgs& a, int s) {   // of a block of sequence s
   if (s >= a.n_seq) return 0;
   FewWalk w;

@@ -86,12 +86,14 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a) {
 
 // The same by pieces of 16 bytes, a block per row: a thread has one piece of a head (of a rotated part in halves one of either half) and waits for it while the block works
 // out the row's sines, rot / 2 of them for all heads. Bound by HBM, with waits in a row's life that only other rows on the SM can fill: 32 registers, so that 2048
-// threads are there. 32768 rows of 32 heads of 128: 105 us = 5.1 TB/s, 0.79 of a copy's rate (two rows per block 109, four 119; blocks that stay and fetch the next
-// row ahead 100 to 108). 16384 rows of 28 + 2 x 4 heads appended: 65 us = 4.6 TB/s (66 to 78).
+// threads are there. 32768 rows of 32 heads of 128: 82 us = 6.5 TB/s, the rate of a copy (102 with the factors side by side; two rows per block, or blocks that stay and
+// fetch the next row ahead, had been no faster then). 16384 rows of 28 + 2 x 4 heads appended: 57 us = 5.3 TB/s (65).
 template <typename TT, bool HALVES>
 __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs a, int lanes_log2) {
   constexpr int V = 16 / (int)sizeof(TT);                // elements of a piece
-  __shared__ float2 cs[128];
+  // Factors of a piece, 16 bytes more between pieces: lanes that read 64 or 32 bytes apart would meet on the same banks (four wavefronts instead of one).
+  constexpr int kPer = HALVES ? V : V / 2, kPitch = kPer == 2 ? 2 : kPer + 2;
+  __shared__ __align__(16) float2 cs[128 / kPer * kPitch];
   __shared__ long long place;
   const int t = blockIdx.x, half = a.rot / 2;
   const int j = threadIdx.x & ((1 << lanes_log2) - 1), step = blockDim.x >> lanes_log2;
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
     if (HALVES && turns_here) v = *reinterpret_cast<const uint4*>(row + (long long)h * a.head + half);
   };
   if (h < a.heads) load();
-  for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i] = rotary_factor(a, a.pos[t], i);
+  for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i / kPer * kPitch + i % kPer] = rotary_factor(a, a.pos[t], i);
   if (a.pool != nullptr && threadIdx.x == 0) place = rotary_place(a, t);
   __syncthreads();
   while (h < a.heads) {
@@ -115,11 +117,13 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
     if (dst != nullptr) {
       if (turns_here && h < a.turned) {
         TT* const eu = reinterpret_cast<TT*>(&u);
+        const float4* const factors = reinterpret_cast<const float4*>(cs + j * kPitch);
         if constexpr (HALVES) {
           TT* const ev = reinterpret_cast<TT*>(&v);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float2 f = cs[j * V + i];
+            const float4 two = factors[i / 2];
+            const float2 f = i % 2 == 0 ? make_float2(two.x, two.y) : make_float2(two.z, two.w);
             const float x = rotary_load(eu + i), y = rotary_load(ev + i);
             rotary_store(eu + i, x * f.x - y * f.y);
             rotary_store(ev + i, y * f.x + x * f.y);
@@ -127,7 +131,8 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
         } else {
 #pragma unroll
           for (int i = 0; i < V; i += 2) {
-            const float2 f = cs[(j * V + i) / 2];
+            const float4 two = factors[i / 4];
+            const float2 f = i % 4 == 0 ? make_float2(two.x, two.y) : make_float2(two.z, two.w);
             const float x = rotary_load(eu + i), y = rotary_load(eu + i + 1);
             rotary_store(eu + i, x * f.x - y * f.y);
             rotary_store(eu + i + 1, y * f.x + x * f.y);
