@@ -87,14 +87,14 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a) {
 // The same by pieces of 16 bytes, a block per row: a thread has one piece of a head (of a rotated part in halves one of either half) and waits for it while the block works
 // out the row's sines, rot / 2 of them for all heads. Bound by HBM, with waits in a row's life that only other rows on the SM can fill: 32 registers, so that 2048
 // threads are there. 32768 rows of 32 heads of 128: 82 us = 6.5 TB/s, the rate of a copy (102 with the factors side by side; two rows per block, or blocks that stay and
-// fetch the next row ahead, had been no faster then). 16384 rows of 28 + 2 x 4 heads appended: 57 us = 5.3 TB/s (65).
+// fetch the next row ahead, had been no faster then). 16384 rows of 28 + 2 x 4 heads appended: 51 us = 5.9 TB/s (57 where the whole
+// block waits for the row's place in the cache, which is only the business of those who store there).
 template <typename TT, bool HALVES>
 __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs a, int lanes_log2) {
   constexpr int V = 16 / (int)sizeof(TT);                // elements of a piece
   // Factors of a piece, 16 bytes more between pieces: lanes that read 64 or 32 bytes apart would meet on the same banks (four wavefronts instead of one).
   constexpr int kPer = HALVES ? V : V / 2, kPitch = kPer == 2 ? 2 : kPer + 2;
   __shared__ __align__(16) float2 cs[128 / kPer * kPitch];
-  __shared__ long long place;
   const int t = blockIdx.x, half = a.rot / 2;
   const int j = threadIdx.x & ((1 << lanes_log2) - 1), step = blockDim.x >> lanes_log2;
   const int turning = (HALVES ? half : a.rot) / V;       // pieces of a head that are rotated (HALVES: together with their partners)
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
   };
   if (h < a.heads) load();
   for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i / kPer * kPitch + i % kPer] = rotary_factor(a, a.pos[t], i);
-  if (a.pool != nullptr && threadIdx.x == 0) place = rotary_place(a, t);
+  const long long place = a.pool != nullptr && h < a.heads && (h >= a.hq || h + step < a.heads) ? rotary_place(a, t) : 0;
   __syncthreads();
   while (h < a.heads) {
     TT* dst = static_cast<TT*>(a.y) + t * a.ldy + (long long)h * a.head + at;
