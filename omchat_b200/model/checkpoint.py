@@ -16,13 +16,14 @@ from __future__ import annotations
 import glob
 import json
 import os
+import warnings
 from dataclasses import fields
 from typing import Dict, Optional, Tuple
 
 import torch
 
 from ..config import FofisunConfig, InternVisionConfig, MunevikConfig, OmChatQwen2Config, OmChatQwen2MoeConfig, SorupelConfig, TifisunConfig, VefunexConfig, VoduzenConfig
-from ..rope import kind
+from ..rope import KINDS, kind
 
 _TEXT_KEYS = ("vocab_size", "hidden_size", "intermediate_size", "num_hidden_layers", "num_attention_heads",
               "num_key_value_heads", "rms_norm_eps", "rope_theta", "max_position_embeddings", "rope_scaling")
@@ -61,6 +62,12 @@ def config_from_dict(d: dict) -> OmChatQwen2Config:
             kw["rope_theta"] = rope["rope_theta"]
         if kind(rope) != "default":
             kw.setdefault("rope_scaling", {k: v for k, v in rope.items() if k != "rope_theta"})
+    scaling = kw.get("rope_scaling")
+    if scaling and kind(scaling) not in KINDS:  # e.g. dynamic, which changes nothing up to max_position_embeddings
+        warnings.warn(f"rope_scaling of type {kind(scaling)!r} is not built ({', '.join(KINDS[1:])} are): positions turn as without it", RuntimeWarning, stacklevel=2)
+        del kw["rope_scaling"]
+    elif scaling and kind(scaling) in ("yarn", "llama3") and scaling.get("original_max_position_embeddings") is None and text.get("max_position_embeddings"):
+        kw["rope_scaling"] = {**scaling, "original_max_position_embeddings": text["max_position_embeddings"]}
     for k in _MM_KEYS:
         if d.get(k) is not None:
             kw[k] = d[k]

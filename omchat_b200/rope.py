@@ -8,6 +8,9 @@ from typing import Optional, Tuple
 import torch
 
 
+KINDS = ("default", "linear", "yarn", "llama3")
+
+
 def _number(scaling: dict, key: str, default: Optional[float] = None) -> float:
     v = scaling.get(key, default)
     if v is None:
@@ -63,5 +66,5 @@ def frequencies(rot_dims: int, theta: float, scaling: Optional[dict] = None, dev
             return x / factor * (1.0 - part) + x * part
         f = [mixed(x) for x in f]
     elif what != "default":
-        raise NotImplementedError(f"rope_scaling of type {what!r} (built: linear, yarn, llama3)")
+        raise NotImplementedError(f"rope_scaling of type {what!r} (built: {', '.join(KINDS[1:])})")
     return torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=device), m

@@ -83,6 +83,19 @@ def test_config_json(tmp_path, hub):
     assert config_from_dict({"rope_parameters": {"rope_theta": 1e4, "rope_type": "default"}}).rope_scaling is None
 
 
+@pytest.mark.parametrize("d", [{"rope_scaling": {"type": "dynamic", "factor": 2.0}}, {"rope_parameters": {"rope_type": "longrope", "rope_theta": 1e4}}])
+def test_kinds_that_are_not_built_change_nothing(d):
+    with pytest.warns(RuntimeWarning, match="not built"):
+        assert config_from_dict(d).rope_scaling is None
+
+
+def test_the_trained_span_is_that_of_the_config():
+    given = {"type": "yarn", "factor": 2.0}
+    assert config_from_dict({"max_position_embeddings": 4096, "rope_scaling": given}).rope_scaling == {**given, "original_max_position_embeddings": 4096}
+    own = {**given, "original_max_position_embeddings": 512}
+    assert config_from_dict({"max_position_embeddings": 4096, "rope_scaling": own}).rope_scaling == own
+
+
 def test_auto_config_keeps_it():
     import omchat_b200.hf as H
     scaling = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
