@@ -3,9 +3,11 @@
 //
 // A wrapper of 25 arguments spent some 10 us in ctypes, in one data_ptr() call per tensor and in the device checks, more than the launch itself.
 #include <Python.h>
+#include <ATen/ops/empty.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <stdint.h>
 #include <string.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -139,6 +141,66 @@ PyObject* need_cuda(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// A tensor argument of the dtype, or null (of another dtype, or no tensor).
+const at::Tensor* of_type(PyObject* t, PyObject* dtype) {
+  if (!THPVariable_Check(t) || !THPDtype_Check(dtype)) return nullptr;
+  const at::Tensor& x = THPVariable_Unpack(t);
+  return x.scalar_type() == reinterpret_cast<THPDtype*>(dtype)->scalar_type ? &x : nullptr;
+}
+
+// rows(tensor, rows, columns, dtype): the row stride of [rows, columns] of dtype with the elements of a row side by side (of one row: the columns), None for any other tensor
+PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  try {
+    const at::Tensor* x = n == 4 ? of_type(args[0], args[3]) : nullptr;
+    const long long r = n == 4 ? PyLong_AsLongLong(args[1]) : 0, c = n == 4 ? PyLong_AsLongLong(args[2]) : 0;
+    if (PyErr_Occurred()) return nullptr;
+    if (x == nullptr || x->dim() != 2 || x->size(0) != r || x->size(1) != c || x->stride(1) != 1) Py_RETURN_NONE;
+    return PyLong_FromLongLong(r > 1 ? x->stride(0) : c);
+  } catch (const std::exception& x) {
+    PyErr_SetString(PyExc_RuntimeError, x.what());
+    return nullptr;
+  }
+}
+
+// contiguous(tensor, dtype, dimensions): its sizes, None where it is not all of that
+PyObject* contiguous(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  try {
+    const at::Tensor* x = n == 3 ? of_type(args[0], args[1]) : nullptr;
+    const long long dims = n == 3 ? PyLong_AsLongLong(args[2]) : 0;
+    if (PyErr_Occurred()) return nullptr;
+    if (x == nullptr || x->dim() != dims || !x->is_contiguous()) Py_RETURN_NONE;
+    PyObject* sizes = PyTuple_New((Py_ssize_t)dims);
+    for (long long i = 0; sizes != nullptr && i < dims; ++i) {
+      PyObject* size = PyLong_FromLongLong(x->size(i));
+      if (size == nullptr) {
+        Py_DECREF(sizes);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(sizes, (Py_ssize_t)i, size);
+    }
+    return sizes;
+  } catch (const std::exception& x) {
+    PyErr_SetString(PyExc_RuntimeError, x.what());
+    return nullptr;
+  }
+}
+
+// new_rows(tensor, rows, columns): what tensor.new_empty((rows, columns)) gives
+PyObject* new_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  try {
+    if (n != 3 || !THPVariable_Check(args[0])) {
+      PyErr_SetString(PyExc_TypeError, "a tensor, rows and columns are wanted");
+      return nullptr;
+    }
+    const long long r = PyLong_AsLongLong(args[1]), c = PyLong_AsLongLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    return THPVariable_Wrap(at::empty({r, c}, THPVariable_Unpack(args[0]).options()));
+  } catch (const std::exception& x) {
+    PyErr_SetString(PyExc_RuntimeError, x.what());
+    return nullptr;
+  }
+}
+
 PyObject* set_error_type(PyObject*, PyObject* type) {
   Py_INCREF(type);
   Py_XSETREF(error_type, type);
@@ -147,6 +209,9 @@ PyObject* set_error_type(PyObject*, PyObject* type) {
 
 PyMethodDef methods[] = {{"entry", make_entry, METH_VARARGS, nullptr},
                          {"need_cuda", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(need_cuda)), METH_FASTCALL, nullptr},
+                         {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rows)), METH_FASTCALL, nullptr},
+                         {"contiguous", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(contiguous)), METH_FASTCALL, nullptr},
+                         {"new_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(new_rows)), METH_FASTCALL, nullptr},
                          {"set_error_type", set_error_type, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "omc_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

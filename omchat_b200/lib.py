@@ -555,22 +555,27 @@ _I32, _F64, _BF16 = torch.int32, torch.float64, torch.bfloat16
 
 def _rows(t: torch.Tensor, rows: int, cols: int, dtype, what: str) -> int:
     """The row stride of t, which is [rows, cols] of dtype with the elements of a row side by side (of one row: any number would do)."""
-    if t.dtype is not dtype or t.shape != (rows, cols) or t.stride(1) != 1:
+    ld = native.rows(t, rows, cols, dtype)
+    if ld is None:
         raise OmcError(f"{what} is {dtype} [{rows}, {cols}] with the elements of a row side by side, not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
-    return t.stride(0) if rows > 1 else cols
+    return ld
 
 
-def _vector(t: torch.Tensor, n: int, dtype, what: str):
-    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
-        raise OmcError(f"{what} is contiguous {dtype} [{n}], not {t.dtype} {tuple(t.shape)}")
+def _vector(t: torch.Tensor, n: Optional[int], dtype, what: str) -> int:
+    size = native.contiguous(t, dtype, 1)
+    if size is None or n is not None and size[0] != n:
+        raise OmcError(f"{what} is contiguous {dtype} [{'any' if n is None else n}], not {t.dtype} {tuple(t.shape)}")
+    return size[0]
 
 
 def _paged(kv_pool: torch.Tensor, block_table: torch.Tensor):
-    if kv_pool.dtype is not _BF16 or kv_pool.dim() != 5 or kv_pool.shape[1] != 2 or not kv_pool.is_contiguous():
+    """(pages, kv heads, page, head) of the pool, (sequences, pages) of the table."""
+    pool, table = native.contiguous(kv_pool, _BF16, 5), native.contiguous(block_table, _I32, 2)
+    if pool is None or pool[1] != 2:
         raise OmcError("the pool is contiguous bfloat16 [pages, 2, kv heads, page, head]")
-    if block_table.dtype is not _I32 or block_table.dim() != 2 or not block_table.is_contiguous():
+    if table is None:
         raise OmcError("the block table is contiguous int32 [sequences, pages]")
-    return kv_pool.shape
+    return pool, table
 
 
 def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, head_dim: int, *, halves: bool = True, back: bool = False,
@@ -583,10 +588,9 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, 
         raise OmcError(f"rotary: rows of bfloat16 or float32, not {dtype}")
     ldx = _rows(x, T, heads * head_dim, dtype, "rotary: x")
     _vector(pos, T, _I32, "rotary: pos")
-    n = turns.numel()
-    _vector(turns, n, _F64, "rotary: turns")
+    n = _vector(turns, None, _F64, "rotary: turns")
     if out is None:
-        out, ldy = x.new_empty((T, heads * head_dim)), heads * head_dim
+        out, ldy = native.new_rows(x, T, heads * head_dim), heads * head_dim
     else:
         ldy = _rows(out, T, heads * head_dim, dtype, "rotary: out")
     rc = load().omc_rotary_rows(x, 0 if dtype is _BF16 else 1, ldx, pos, T, heads, head_dim, turns, 2 * n, 1 if halves else 0, 1 if back else 0, mscale, out, ldy,
@@ -601,21 +605,19 @@ def rotary_kv_append(qkv: torch.Tensor, pos: torch.Tensor, seq_ids: Optional[tor
     cache rows (seq_ids[t], pos[t]) of kv_pool [pages, 2, Hkv, page, head]. Rows without a place in the table (sequence -1: padding) are not appended; no two
     rows may have the same place."""
     _need_cuda(qkv, pos, seq_ids, turns, kv_pool, block_table, q_out)
-    n_pages, _, Hkv, page, head = _paged(kv_pool, block_table)
+    (n_pages, _, Hkv, page, head), (n_seq, max_pages) = _paged(kv_pool, block_table)
     T = qkv.shape[0]
     ld = _rows(qkv, T, (Hq + 2 * Hkv) * head, _BF16, "rotary_kv_append: qkv")
     _vector(pos, T, _I32, "rotary_kv_append: pos")
     if seq_ids is not None:
         _vector(seq_ids, T, _I32, "rotary_kv_append: seq_ids")
-    n = turns.numel()
-    _vector(turns, n, _F64, "rotary_kv_append: turns")
+    n = _vector(turns, None, _F64, "rotary_kv_append: turns")
     if q_out is None:
-        q_out, ldq = qkv.new_empty((T, Hq * head)), Hq * head
+        q_out, ldq = native.new_rows(qkv, T, Hq * head), Hq * head
     else:
         ldq = _rows(q_out, T, Hq * head, _BF16, "rotary_kv_append: q_out")
     rc = load().omc_rotary_kv_append(qkv, ld, pos, seq_ids, T, Hq, Hkv, head, turns, 2 * n, 1 if halves else 0, mscale, q_out,
-                                     ldq, kv_pool, n_pages, block_table, block_table.shape[0],
-                                     block_table.shape[1], page, _stream())
+                                     ldq, kv_pool, n_pages, block_table, n_seq, max_pages, page, _stream())
     _check(rc, "omc_rotary_kv_append")
     return q_out
 
@@ -626,14 +628,13 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
     the last positions of the ctx_lens[s] that sequence s has. max_new / max_ctx: what no sequence has more of (host numbers; the lengths
     themselves stay on the device). Rows behind cu_new[-1] are not written. out may be q."""
     _need_cuda(q, kv_pool, block_table, cu_new, ctx_lens, out)
-    n_pages, _, Hkv, page, head = _paged(kv_pool, block_table)
-    n_seq, max_pages = block_table.shape
+    (n_pages, _, Hkv, page, head), (n_seq, max_pages) = _paged(kv_pool, block_table)
     T = q.shape[0]
     ldq = _rows(q, T, Hq * head, _BF16, "paged_attention: q")
     _vector(cu_new, n_seq + 1, _I32, "paged_attention: cu_new")
     _vector(ctx_lens, n_seq, _I32, "paged_attention: ctx_lens")
     if out is None:
-        out, ldo = q.new_empty((T, Hq * head)), Hq * head
+        out, ldo = native.new_rows(q, T, Hq * head), Hq * head
     else:
         ldo = _rows(out, T, Hq * head, _BF16, "paged_attention: out")
     L = load()

@@ -94,6 +94,27 @@ def need_cuda(error: type):
     return check
 
 
+def rows(t: torch.Tensor, n: int, cols: int, dtype) -> Optional[int]:
+    """The row stride of t if it is [n, cols] of dtype with the elements of a row side by side (of one row any number would do: cols), else None."""
+    if _module is not None:
+        return _module.rows(t, n, cols, dtype)
+    if t.dtype is not dtype or t.shape != (n, cols) or t.stride(1) != 1:
+        return None
+    return t.stride(0) if n > 1 else cols
+
+
+def contiguous(t: torch.Tensor, dtype, dims: int) -> Optional[tuple]:
+    """The sizes of t if it is contiguous, of dtype and has so many dimensions, else None."""
+    if _module is not None:
+        return _module.contiguous(t, dtype, dims)
+    return tuple(t.shape) if t.dtype is dtype and t.dim() == dims and t.is_contiguous() else None
+
+
+def new_rows(like: torch.Tensor, n: int, cols: int) -> torch.Tensor:
+    """like.new_empty((n, cols))."""
+    return _module.new_rows(like, n, cols) if _module is not None else like.new_empty((n, cols))
+
+
 def raw_stream() -> int:
     """The current stream of the current device."""
     return torch.cuda.current_stream().cuda_stream
