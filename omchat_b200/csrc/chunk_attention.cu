@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(kCaThreads, 1) chunk_attn_kernel(const ChunkAr
   CaShared* const sh = reinterpret_cast<CaShared*>(ring + 2 * C::kSlots * C::kTile);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rep = a.Hq / a.Hkv;
   pdl_launch();
+  pdl_wait();
   const WaitReport report{&sh->dead, &g_chunk_failures, a.failed};
   if (warp < 2) ca_span(a, sh, rep, lane, warp == 1);
   if (warp == 12) {
@@ -818,7 +819,18 @@ static int ca_launch(const ChunkArgs& a, const CaPlan& plan, cudaStream_t st) {
     if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
     done[dev] = true;
   }
-  chunk_attn_kernel<D><<<plan.grid, kCaThreads, CaShape<D>::kSmem, st>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(plan.grid);
+  cfg.blockDim = dim3(kCaThreads);
+  cfg.dynamicSmemBytes = CaShape<D>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel<D>, a);
+  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   const int rc = check_launch("omc_paged_chunk_attn");
   return rc != OMC_OK || !plan.cut ? rc : ca_join<D>(a, plan, st);
 }

@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kP
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.Hq / a.Hkv, cta = blockIdx.x;
   pdl_launch();
+  pdl_wait();
   // ------------------------------------------------------------------------------------------------ the CTA's part, found by every warp for itself
   FewWalk w;
   int first_tile;
@@ -522,12 +523,14 @@ static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
   cfg.blockDim = dim3(FewShape<D, MT>::kThreads);
   cfg.dynamicSmemBytes = FewShape<D, MT>::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = kShared && a.cluster > 1 ? 1 : 0;
+  cfg.numAttrs = kShared && a.cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_kernel<D, MT, kShared>, a);
   if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");

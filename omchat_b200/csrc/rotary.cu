@@ -57,6 +57,8 @@ template <typename TT>
 __global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a) {
   const int t = blockIdx.x, half = a.rot / 2;
   __shared__ float2 cs[128];
+  pdl_launch();
+  pdl_wait();
   for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i] = rotary_factor(a, a.pos[t], i);
   __syncthreads();
   const TT* row = static_cast<const TT*>(a.x) + t * a.ldx;
@@ -99,6 +101,8 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
   const int j = threadIdx.x & ((1 << lanes_log2) - 1), step = blockDim.x >> lanes_log2;
   const int turning = (HALVES ? half : a.rot) / V;       // pieces of a head that are rotated (HALVES: together with their partners)
   const bool turns_here = j < turning;
+  pdl_launch();
+  pdl_wait();
   const int at = turns_here ? j * V : a.rot + (j - turning) * V;
   const TT* const row = static_cast<const TT*>(a.x) + t * a.ldx + at;
   int h = j < turning + (a.head - a.rot) / V ? threadIdx.x >> lanes_log2 : a.heads;   // the threads beyond a head's pieces have none
@@ -147,6 +151,23 @@ __global__ void __launch_bounds__(512, 4) rotary_pieces_kernel(const RotaryArgs 
   }
 }
 
+// A grid of `blocks` that may be launched while the one in front still runs: the kernels wait for it before anything else.
+template <typename... Args>
+static int rotary_start(void (*kernel)(Args...), int blocks, int threads, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
+  return check_launch("omc_rotary");
+}
+
 // 16-byte pieces: everything on such boundaries, and none with rotated elements beside others.
 template <typename TT>
 static bool rotary_by_pieces(const RotaryArgs& a) {
@@ -162,16 +183,12 @@ static int rotary_pieces_launch(const RotaryArgs& a, cudaStream_t st) {
   while ((1 << log2) < pieces) ++log2;
   const long long all = (long long)a.heads << log2;
   const int threads = all >= 512 ? 512 : (int)(all + 31) / 32 * 32;   // all heads of a row at once where a block can
-  if (a.halves) rotary_pieces_kernel<TT, true><<<a.T, threads, 0, st>>>(a, log2);
-  else rotary_pieces_kernel<TT, false><<<a.T, threads, 0, st>>>(a, log2);
-  return check_launch("omc_rotary");
+  return a.halves ? rotary_start(rotary_pieces_kernel<TT, true>, a.T, threads, st, a, log2) : rotary_start(rotary_pieces_kernel<TT, false>, a.T, threads, st, a, log2);
 }
 
 static int rotary_launch(const RotaryArgs& a, bool fp32, cudaStream_t st) {
   if (fp32 ? rotary_by_pieces<float>(a) : rotary_by_pieces<bf16>(a)) return fp32 ? rotary_pieces_launch<float>(a, st) : rotary_pieces_launch<bf16>(a, st);
-  if (fp32) rotary_rows_kernel<float><<<a.T, 256, 0, st>>>(a);
-  else rotary_rows_kernel<bf16><<<a.T, 256, 0, st>>>(a);
-  return check_launch("omc_rotary");
+  return fp32 ? rotary_start(rotary_rows_kernel<float>, a.T, 256, st, a) : rotary_start(rotary_rows_kernel<bf16>, a.T, 256, st, a);
 }
 
 static int rotary_check(int T, int head, int rot, const double* turns) {
