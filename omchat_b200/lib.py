@@ -583,7 +583,7 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, turns: torch.Tensor, heads: int, 
     """Rotary positions of rows x [T, heads * head_dim] (bf16 or fp32, row-strided) at positions pos (int32 [T]); out may be x. turns: float64
     [rotated dims / 2], see rope.frequencies(); halves: pairs (i, i + rotated / 2) instead of (2i, 2i + 1); back: by the negative angle."""
     _need_cuda(x, pos, turns, out)
-    dtype, T = x.dtype, x.shape[0]
+    dtype, T = x.dtype, x.size(0)
     if dtype is not _BF16 and dtype is not torch.float32:
         raise OmcError(f"rotary: rows of bfloat16 or float32, not {dtype}")
     ldx = _rows(x, T, heads * head_dim, dtype, "rotary: x")
@@ -606,7 +606,7 @@ def rotary_kv_append(qkv: torch.Tensor, pos: torch.Tensor, seq_ids: Optional[tor
     rows may have the same place."""
     _need_cuda(qkv, pos, seq_ids, turns, kv_pool, block_table, q_out)
     (n_pages, _, Hkv, page, head), (n_seq, max_pages) = _paged(kv_pool, block_table)
-    T = qkv.shape[0]
+    T = qkv.size(0)
     ld = _rows(qkv, T, (Hq + 2 * Hkv) * head, _BF16, "rotary_kv_append: qkv")
     _vector(pos, T, _I32, "rotary_kv_append: pos")
     if seq_ids is not None:
@@ -629,7 +629,7 @@ def paged_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.T
     themselves stay on the device). Rows behind cu_new[-1] are not written. out may be q."""
     _need_cuda(q, kv_pool, block_table, cu_new, ctx_lens, out)
     (n_pages, _, Hkv, page, head), (n_seq, max_pages) = _paged(kv_pool, block_table)
-    T = q.shape[0]
+    T = q.size(0)
     ldq = _rows(q, T, Hq * head, _BF16, "paged_attention: q")
     _vector(cu_new, n_seq + 1, _I32, "paged_attention: cu_new")
     _vector(ctx_lens, n_seq, _I32, "paged_attention: ctx_lens")
