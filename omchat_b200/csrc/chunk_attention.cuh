@@ -31,7 +31,8 @@ struct ChunkArgs {
 };
 
 struct CaPlan {
-  int grid, part_rows, cluster;   // cluster: of few rows, CTAs that share a block; 0: the line is cut
+  int grid, part_rows;
+  int cluster, warps;      // of few rows: CTAs that share a block (0: the line is cut), and their warps
   bool few;                // chunk_attention_few.cu has it
   bool cut, fits;          // whether a block can be cut; whether the products can be counted in 31 bits
   long long blocks, bytes; // at most as many blocks; of the workspace

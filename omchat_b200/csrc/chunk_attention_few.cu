@@ -2,19 +2,19 @@
 // the group) of a sequence and key/value head fit one to three tiles of mma.sync.
 //
 // Every key and value is read once and meets few rows, so HBM bounds a large call, and a small one the way from the launch to the first scores. Neither wants
-// tcgen05: for 7 rows an M of 128, tensor memory and the hand-offs between warps cost 12.9 us of a token behind 1087 positions (28 heads on 4 of 128, 2 MB; this kernel 8.0) and 42
-// of 32 tokens behind up to 4096 (175 MB; 34.9, of which 27 at the rate of a copy; all in a graph).
+// tcgen05: for 7 rows an M of 128, tensor memory and the hand-offs between warps cost 12.9 us of a token behind 1087 positions (28 heads on 4 of 128, 2 MB; this kernel 7.0) and 42
+// of 32 tokens behind up to 4096 (175 MB; 34.7, of which 27 at the rate of a copy; all in a graph).
 //
 // Here a warp is a pipeline of its own and waits for nobody: it copies groups of 16 keys (32 of heads of 64) by cp.async into a ring of its own (keys, values, keys, values: 4 KB
 // each), takes the scores with the rows in registers, keeps a maximum, a sum and an output, and the warps of a CTA take the groups of a block in turn. Two CTAs of four
-// warps per SM have 128 KB under way (an SM takes in some 46 bytes a cycle: 1.4 thousand cycles' worth). Where a block ends the warps are merged.
+// warps per SM, or one of eight, have 128 KB under way (an SM takes in some 46 bytes a cycle: 1.4 thousand cycles' worth). Where a block ends the warps are merged.
 //
 // Who has which keys: a block (a sequence's rows of one key/value head) is a cluster's of up to 8 CTAs, which join their parts through each other's shared memory: one launch, no
 // workspace, and no search for a CTA's share. Where that leaves CTAs more than eight tiles of 64 keys (long contexts, or more blocks than fill the GPU evenly) all
 // products lie in one line that is cut evenly, as in chunk_attention.cu, and a second kernel joins: 1 token behind 8000 20.6 us by clusters, 11.7 cut; 32 behind 4096 39.7 and 34.9;
-// 64 behind 2000 37.2 and 35.6; but 8 behind 2000 10.1 and 12.6, one behind 1087 8.0 and 9.7.
+// 64 behind 2000 37.2 and 35.6; but 8 behind 2000 10.1 and 12.6, one behind 1087 8.0 and 9.7 (each with four warps).
 //
-// What a small call is made of (one token behind 1087, cycles): lengths 700, page of the first rows 900, copies 1400 (shared memory's way in), a group 1100 (scores 370, softmax 290,
+// What a small call is made of (one token behind 1087, four warps, cycles): lengths 700, page of the first rows 900, copies 1400 (shared memory's way in), a group 1100 (scores 370, softmax 290,
 // output 330) of up to three per warp, merging 1500 and joining 1300.
 #include <math.h>
 #include <stdint.h>
@@ -27,12 +27,15 @@ namespace omc {
 // Tiles that a CTA has at least where blocks are cut (one token behind 8000: 11.7 us with 2, 12.1 with 3, 12.9 with 4); CTAs of a cluster; tiles per CTA up to which clusters share.
 constexpr int kFewMinUnits = 2, kFewCluster = 8, kFewTiles = 8;
 
-template <int D, int MT>
+template <int D>
+constexpr int kFewGroup = D == 128 ? 16 : 32;   // keys of a group
+
+template <int D, int MT, int WARPS>
 struct FewShape {
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kGroup = D == 128 ? 16 : 32, kPair = 32 / kGroup, kSub = kGroup * D * 2, kSubs = 4, kPitch = D + 8;
+  static constexpr int kWarps = WARPS, kThreads = 32 * kWarps, kGroup = kFewGroup<D>, kPair = 32 / kGroup, kSub = kGroup * D * 2, kSubs = 4, kPitch = D + 8;
   static constexpr int kRing = kWarps * kSubs * kSub, kQueries = MT * 16 * D * 2, kJoint = kWarps * 16 * kPitch * 4;
   static constexpr int kSmem = kRing + kQueries + kJoint + kWarps * 16 * 8;
-  static constexpr int kPerSM = 2;
+  static constexpr int kPerSM = 8 / WARPS;
   static_assert(kPerSM * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -131,9 +134,9 @@ __device__ __forceinline__ float4 few_remote4(uint32_t at, uint32_t cta) {
 }
 
 // kShared: a block is one CTA's or that of a cluster, whose parts are joined through shared memory; else the line is cut.
-template <int D, int MT, bool kShared>
-__global__ void __launch_bounds__(FewShape<D, MT>::kThreads, FewShape<D, MT>::kPerSM) chunk_attn_few_kernel(const ChunkArgs a) {
-  using C = FewShape<D, MT>;
+template <int D, int MT, int WARPS, bool kShared>
+__global__ void __launch_bounds__(FewShape<D, MT, WARPS>::kThreads, FewShape<D, MT, WARPS>::kPerSM) chunk_attn_few_kernel(const ChunkArgs a) {
+  using C = FewShape<D, MT, WARPS>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.Hq / a.Hkv, cta = blockIdx.x;
   pdl_launch();
@@ -498,9 +501,18 @@ bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim,
   p.few = true;
   p.blocks = blocks;
   p.part_rows = (int)rows;
-  p.cluster = 1;
-  while (p.cluster < kFewCluster && p.cluster < tiles && blocks * p.cluster * 2 <= slots) p.cluster *= 2;
-  p.cut = tiles > kFewTiles * p.cluster + kFewTiles / 2;
+  // CTAs of a block, with four warps (two CTAs per SM) and with eight (one, and fewer clusters at a time: a cluster lies in one of the GPU's groups of some 18 SMs)
+  const int per_tile = kCaKeys / (head_dim == 128 ? kFewGroup<128> : kFewGroup<64>);
+  auto rounds = [&](int cluster, int warps) { return ((tiles + cluster - 1) / cluster * per_tile + warps - 1) / warps; };   // groups a warp has
+  int four = 1, eight = 1;
+  while (four < kFewCluster && four < tiles && blocks * four * 2 <= slots) four *= 2;
+  while (eight < kFewCluster && eight < tiles && blocks * eight * 2 <= (eight == 1 ? 128 : eight == 2 ? 96 : 64)) eight *= 2;
+  // One token behind 2000 7.6 us with eight warps, 8.4 with four; 32 behind 512, where eight warps need no cluster, 8.4 and 10.0; but 4 behind 4000 14.6 and 13.3 with as many groups
+  // a warp either way.
+  const bool wide = blocks <= num_sms() && (rounds(eight, 8) < rounds(four, 4) || (rounds(eight, 8) == rounds(four, 4) && eight == 1 && four > 1));
+  p.warps = wide ? 8 : 4;
+  p.cluster = wide ? eight : four;
+  p.cut = tiles > kFewTiles * p.cluster * (p.cluster == 1 ? p.warps / 4 : 1) + kFewTiles / 2;
   if (p.cut && rows * head_dim > 2048) return false;
   if (p.cut) p.cluster = 0;
   const long long parts = p.cut ? most / kFewMinUnits : blocks * p.cluster;
@@ -509,19 +521,19 @@ bool few_plan(int n_seq, int Hkv, long long rows, long long tiles, int head_dim,
   return true;
 }
 
-template <int D, int MT, bool kShared>
+template <int D, int MT, int WARPS, bool kShared>
 static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   const int dev = cur_device();
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_few_kernel<D, MT, kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, MT>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(chunk_attn_few_kernel<D, MT, WARPS, kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, MT, WARPS>::kSmem);
     if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
     done[dev] = true;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(FewShape<D, MT>::kThreads);
-  cfg.dynamicSmemBytes = FewShape<D, MT>::kSmem;
+  cfg.blockDim = dim3(FewShape<D, MT, WARPS>::kThreads);
+  cfg.dynamicSmemBytes = FewShape<D, MT, WARPS>::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -531,18 +543,24 @@ static int launch(const ChunkArgs& a, int grid, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kShared && a.cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_kernel<D, MT, kShared>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_attn_few_kernel<D, MT, WARPS, kShared>, a);
   if (e != cudaSuccess) return set_error(OMC_ERR_CUDA, cudaGetErrorString(e));
   return check_launch("omc_paged_chunk_attn");
 }
 
+template <int WARPS>
+static int few_shared(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st) {
+  const int rows = plan.part_rows;
+  if (head_dim == 128) return rows <= 16 ? launch<128, 1, WARPS, true>(a, plan.grid, st) : launch<128, 2, WARPS, true>(a, plan.grid, st);
+  if (rows <= 16) return launch<64, 1, WARPS, true>(a, plan.grid, st);
+  return rows <= 32 ? launch<64, 2, WARPS, true>(a, plan.grid, st) : launch<64, 3, WARPS, true>(a, plan.grid, st);
+}
+
 int few_launch(const ChunkArgs& a, const CaPlan& plan, int head_dim, cudaStream_t st) {
-  const int rows = plan.part_rows, grid = plan.grid;
-  if (a.cluster > 0) {
-    if (head_dim == 128) return rows <= 16 ? launch<128, 1, true>(a, grid, st) : launch<128, 2, true>(a, grid, st);
-    return rows <= 16 ? launch<64, 1, true>(a, grid, st) : rows <= 32 ? launch<64, 2, true>(a, grid, st) : launch<64, 3, true>(a, grid, st);
-  }
-  const int rc = head_dim == 128 ? launch<128, 1, false>(a, grid, st) : rows <= 16 ? launch<64, 1, false>(a, grid, st) : launch<64, 2, false>(a, grid, st);
+  if (a.cluster > 0) return plan.warps == 8 ? few_shared<8>(a, plan, head_dim, st) : few_shared<4>(a, plan, head_dim, st);
+  int rc;
+  if (head_dim == 128) rc = launch<128, 1, 4, false>(a, plan.grid, st);
+  else rc = plan.part_rows <= 16 ? launch<64, 1, 4, false>(a, plan.grid, st) : launch<64, 2, 4, false>(a, plan.grid, st);
   return rc != OMC_OK ? rc : chunk_join(a, plan, head_dim, st);
 }
 

@@ -187,6 +187,7 @@ FEW = [  # calls of few rows a sequence and head: blocks that clusters share, of
     ([4, 1, 3], [700, 2000, 5], 28, 4, 128, 24), ([1] * 60 + [0] * 30 + [1] * 60, [(i * 37) % 3000 + 1 for i in range(150)], 14, 2, 128, 64),
     ([1] * 1100, [800 if i == 700 else i % 90 + 1 for i in range(1100)], 3, 1, 64, 64), ([1], [20000], 4, 4, 64, 64), ([2, 1], [16000, 9], 14, 2, 64, 128), ([1] * 70, [999] * 70, 16, 2, 128, 64),
     ([4] * 40, [(i * 53) % 700 + 4 for i in range(40)], 28, 4, 128, 64), ([6, 6], [400, 77], 8, 1, 64, 64), ([1], [1500], 48, 1, 64, 64), ([1] * 3, [64 * 8, 64 * 8 + 1, 64 * 7], 4, 1, 128, 32),
+    ([5], [900], 14, 2, 64, 16), ([4], [1001], 28, 4, 128, 64), ([1] * 32, [16 * i + 9 for i in range(32)], 28, 4, 128, 64), ([2], [640], 12, 1, 64, 64), ([1], [2048], 2, 2, 64, 64),
 ]
 
 
