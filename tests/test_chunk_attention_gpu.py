@@ -264,3 +264,59 @@ def test_append_then_attend_is_a_prompt_in_portions():
         first += m
     assert first == n
     _check(out, q, pool, table, [n], [n], hq, hkv, head, head ** -0.5)
+
+
+def _step(x, pos, turns, hq, pool, table, cu, lens, n, c):
+    q = lib.rotary_kv_append(x, pos, None, turns, hq, pool, table)
+    return lib.paged_attention(q, pool, table, cu, lens, n, c, hq, 0.088)
+
+
+@pytest.mark.parametrize("n,c", [(1, 700), (3, 5000), (90, 900)])
+def test_right_behind_who_writes(n, c):
+    """The kernels may be launched while the one in front still runs: rows, positions, lengths and pages that it writes are those that they read."""
+    hq, hkv = 14, 2
+    q, pool, table, cu, lens = _inputs([n], [c], hq, hkv, 128, 64, poison=False)
+    g = torch.Generator().manual_seed(n)
+    rows = [torch.randn(n, (hq + 2 * hkv) * 128, generator=g).to(BF).cuda() for _ in range(6)]
+    pos, turns = torch.arange(c - n, c, dtype=torch.int32).cuda(), torch.rand(64, dtype=torch.float64, generator=g).cuda()
+    want = []
+    for x in rows:
+        want.append(_step(x, pos, turns, hq, pool, table, cu, lens, n, c).clone())
+        torch.cuda.synchronize()
+    slow, x, now, len_ = torch.randn(4096, 4096, device="cuda"), torch.empty_like(rows[0]), torch.zeros_like(pos), torch.zeros_like(lens)
+    got = []
+    for r in rows * 3:
+        slow = slow @ slow * 1e-3
+        x.copy_(r)
+        now.copy_(pos)
+        len_.copy_(lens)
+        got.append(_step(x, now, turns, hq, pool, table, cu, len_, n, c))
+        for t in (x, now, len_):
+            t.zero_()                                        # behind it: what they read must have been read
+    for a, b in zip(got, want * 3):
+        assert torch.equal(a, b)
+
+
+def test_a_graph_in_which_streams_meet():
+    hq, hkv, n, c = 14, 2, 2, 3000
+    q, pool, table, cu, lens = _inputs([n], [c], hq, hkv, 128, 64, poison=False)
+    x = torch.randn(n, (hq + 2 * hkv) * 128, generator=torch.Generator().manual_seed(3)).to(BF).cuda()
+    pos, turns = torch.arange(c - n, c, dtype=torch.int32).cuda(), torch.rand(64, dtype=torch.float64).cuda()
+    want = _step(x, pos, turns, hq, pool, table, cu, lens, n, c).clone()
+    side, graph, other = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros(1000, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            first = lib.rotary(x, pos, turns, hq + 2 * hkv, 128)
+        other += 1
+        main.wait_stream(side)
+        second = _step(x, pos, turns, hq, pool, table, cu, lens, n, c)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            third = _step(x, pos, turns, hq, pool, table, cu, lens, n, c)
+        main.wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+    assert torch.equal(second, want) and torch.equal(third, want) and torch.equal(first, lib.rotary(x, pos, turns, hq + 2 * hkv, 128)) and bool((other == 3).all())
