@@ -7,7 +7,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from oracle import omchat_oracle as O  # noqa: E402  (checker only)
+from oracle import omchat_oracle as O  # noqa: E402
 from tiny import TINY, tiny_inputs, tiny_state_dict  # noqa: E402
 from test_model_gpu import check, oracle_cfg, tiny_cfgs  # noqa: E402
 from test_serving_gpu import _same_or_near_tie  # noqa: E402
